@@ -17,6 +17,7 @@ import torch
 from ..parts.kv_pages import K_LAYOUT, V_LAYOUT, key_pages_shape, value_pages_shape
 from ..errors import KernelError, ReplayMismatch
 from . import build
+from .mx4 import SIGNATURES as _MX4_SIGNATURES, Mx4Matrix, Mx4Ops
 
 _F32, _BF16 = 0, 1
 _vp, _i, _f = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
@@ -65,6 +66,7 @@ _SIGNATURES = {
     "llm_peak_copy": [_vp, _vp, ctypes.c_size_t, _i, _vp],
     "llm_peak_mfma_bf16": [_vp, _i, ctypes.POINTER(ctypes.c_double), _vp],
     "llm_peak_fma_f32": [_vp, _i, ctypes.POINTER(ctypes.c_double), _vp],
+    **_MX4_SIGNATURES,
 }
 
 
@@ -97,7 +99,7 @@ class PreparedWeight:
         self.shape, self.dtype = w.shape, w.dtype
 
 
-class HipOps:
+class HipOps(Mx4Ops):
     """The operations of the model on the GPU: the only implementation there is.  Every method
     checks its operands on the host before a kernel is launched."""
 
@@ -505,12 +507,17 @@ class HipOps:
             epilogue, _code(out.dtype), mm, n, k, ldw, k_split, self._stream()), "gemm_skinny_bf16")
 
     def linear(self, x, w, bias, out_dtype, residual=None, then_norm=None):
-        """x W^T (+ bias) as ``out_dtype``.  ``x`` is a matrix or a ``normed`` record.  With
+        """x W^T (+ bias) as ``out_dtype``.  ``x`` is a matrix or a ``normed`` record; with a weight
+        in MXFP4 (``quantize_mx4``, ``mx4_from_codes``) it may be in MXFP4 too.  With
         ``residual`` (the float32 stream, same shape as the result) the product is added into it
         where the kernel can do that, and None is returned; otherwise the result is returned and
         the caller adds it.  ``then_norm`` = (weight, eps) says that an RMS norm with these reads
         ``residual`` next, before anything else touches it: where the product adds into the
         stream at up to ``ACCUM_ROWS`` rows it then returns a ``Prenormed`` for ``normed``."""
+        if isinstance(w, Mx4Matrix):
+            return self._linear_mx4(x, w, bias, out_dtype, residual)
+        if isinstance(x, Mx4Matrix):
+            raise KernelError("linear: rows in MXFP4 need a weight in MXFP4")
         lazy = isinstance(x, NormedRows)
         m, k = (x.n_rows, x.res.shape[1]) if lazy else x.shape
         n, k2 = w.shape
@@ -658,6 +665,10 @@ class HipOps:
         another of ``ACTIVATIONS``: one kernel where a product of ours takes the rows, else the
         library's product followed by the kernel that gates.  ``x`` is a matrix or a ``normed``
         record; ``dtype`` is the activation dtype (needed for a record)."""
+        if isinstance(w, Mx4Matrix):
+            return self._linear_swiglu_mx4(x, w, dtype, activation)
+        if isinstance(x, Mx4Matrix):
+            raise KernelError("linear_swiglu: rows in MXFP4 need a weight in MXFP4")
         gated = self._EPI_SWIGLU | (self._act(activation) << 4)
         lazy = isinstance(x, NormedRows)
         m, k = (x.n_rows, x.res.shape[1]) if lazy else x.shape

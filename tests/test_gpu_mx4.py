@@ -1,0 +1,401 @@
+"""Matrices in MXFP4 and their products against plain implementations in float64: a quantiser, a
+reader of the tiles and a product written here with numpy, from the format's definition."""
+import numpy as np
+import pytest
+import torch
+
+from libllm_amd.errors import KernelError
+
+pytestmark = pytest.mark.gpu
+
+GRID = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0])
+HALF_BF16, HALF_F32 = 2.0 ** -8, 2.0 ** -24        # the most a rounding is off, relative to the value
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from libllm_amd.hip import HipOps
+    return HipOps()
+
+
+# ------------------------------------------------------------------------------- plain forms
+def quantise(x):
+    """Codes [m, k] and scales [m, ceil(k / 32)] of a float64 matrix, block by block."""
+    x = np.asarray(x, dtype=np.float64)
+    m, k = x.shape
+    blocks = -(-k // 32)
+    codes = np.zeros((m, k), dtype=np.uint8)
+    scales = np.zeros((m, blocks), dtype=np.uint8)
+    for b in range(blocks):
+        part = x[:, 32 * b:32 * b + 32]
+        top = np.abs(part).max(axis=1)
+        bad = ~np.isfinite(part).all(axis=1)
+        _, e = np.frexp(np.where(bad | (top == 0), 1.0, top))       # top = f 2^e with f in [0.5, 1)
+        s = np.maximum(np.where(top == 0, -127, e - 1 - 2), -127)
+        a = np.ldexp(np.abs(np.where(np.isfinite(part), part, 0.0)), -s[:, None])
+        # the nearest of the grid; at equal distance the one whose code is even
+        d = np.abs(a[:, :, None] - GRID)
+        near = d == d.min(axis=2, keepdims=True)
+        pick = np.where(near, np.arange(8) % 2 * 8 + np.arange(8), 99).argmin(axis=2)
+        codes[:, 32 * b:32 * b + 32] = pick + 8 * np.signbit(part)
+        scales[:, b] = np.where(bad, 255, s + 127)
+    return codes, scales
+
+
+def values(codes, scales):
+    k = codes.shape[1]
+    v = np.where(codes > 7, -1.0, 1.0) * GRID[codes & 7]
+    s = np.ldexp(1.0, scales.astype(np.int64) - 127)
+    s = np.where(scales == 255, np.nan, s)
+    return v * np.repeat(s, 32, axis=1)[:, :k]
+
+
+def file_form(codes, scales):
+    """Two codes a byte, the even element in the low half."""
+    if codes.shape[1] % 2:
+        codes = np.pad(codes, ((0, 0), (0, 1)))
+    return torch.from_numpy(codes[:, 0::2] | (codes[:, 1::2] << 4)), torch.from_numpy(scales)
+
+
+def rows_of(q):
+    """(codes, scales) by rows, read out of the tiles by the layout's definition (csrc/mx4.h)."""
+    m, k = q.shape
+    tiles, units = -(-m // 16), -(-k // 128)
+    quads = -(-units // 4)
+    c = q.codes.cpu().numpy().reshape(tiles, units, 4, 16, 16)            # tile, unit, block, row, byte
+    c = np.stack([c & 15, c >> 4], axis=-1).reshape(tiles, units, 4, 16, 32)
+    c = c.transpose(0, 3, 1, 2, 4).reshape(tiles * 16, units * 128)
+    s = q.scales.cpu().numpy().reshape(tiles, quads, 4, 16, 4)            # tile, quad, block, row, unit of the quad
+    s = s.transpose(0, 3, 1, 4, 2).reshape(tiles * 16, quads * 16)[:, :units * 4]
+    return c, s
+
+
+def normal(shape, seed, scale=1.0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype)
+
+
+def weight(n, k, seed):
+    codes, scales = quantise(normal((n, k), seed, k ** -0.5).double().numpy())
+    return codes, scales, values(codes, scales)
+
+
+def bound(x, w, k, dtype):
+    """What a product summed in 32 bits may be off by, per element.  Products of bfloat16 and MXFP4
+    numbers (8 and 2 bits) are exact in 32 bits; k of them are added, in whatever order, by at most
+    k additions, each off by at most 2^-24 of a partial sum, which is at most sum |x| |w|.  The
+    matrix cores may cut off instead of rounding: twice that.  Then one rounding of the result."""
+    magnitude = np.abs(x) @ np.abs(w).T
+    exact = np.abs(x @ w.T)
+    err = 2 * k * HALF_F32 * magnitude
+    half = HALF_BF16 if dtype == torch.bfloat16 else HALF_F32
+    return err + half * (exact + err) + 1e-38
+
+
+def gate(act, g, u):
+    if act == "relu":
+        return np.maximum(g, 0) * u
+    if act == "gelu_tanh":
+        return 0.5 * g * (1 + np.tanh(np.sqrt(2 / np.pi) * (g + 0.044715 * g ** 3))) * u
+    return g / (1 + np.exp(-g)) * u
+
+
+# ------------------------------------------------------------------------------- conversions
+SIZES = [(1, 1), (1, 32), (2, 31), (3, 33), (16, 128), (17, 129), (5, 500), (40, 512), (33, 1030), (130, 96)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,k", SIZES)
+def test_quantize(ops, m, k, dtype):
+    x = normal((m, k), 100 * m + k, 3.0, dtype)
+    x[0, 0] = 0.0
+    if m > 2:
+        x[1] = 0.0
+        x[2] *= 2.0 ** -100
+    codes, scales = quantise(x.double().numpy())
+    q = ops.quantize_mx4(x.cuda())
+    assert q.shape == (m, k)
+    got_codes, got_scales = rows_of(q)
+    blocks = scales.shape[1]
+    assert np.array_equal(got_scales[:m, :blocks], scales)
+    assert np.array_equal(got_codes[:m, :k], codes)
+    # what pads the tiles is zero
+    assert not got_codes[m:].any() and not got_codes[:, k:].any()
+    assert not got_scales[m:].any() and not got_scales[:, blocks:].any()
+    for out in (torch.float32, torch.bfloat16):
+        back = ops.dequantize_mx4(q, out)
+        assert back.dtype == out and back.shape == (m, k)
+        assert np.array_equal(back.double().cpu().numpy(), values(codes, scales))
+
+
+def test_quantize_ties_limits_and_signs(ops):
+    # one block per row, its largest magnitude 4 .. 8 in units of the scale
+    ties = [0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 7.0, 7.99, 4.0]
+    row = np.zeros(32)
+    row[:10], row[10:20] = ties, [-t for t in ties]
+    row[20] = -0.0
+    above = np.nextafter(row.astype(np.float32), np.float32(np.inf)).astype(np.float64)
+    below = np.nextafter(row.astype(np.float32), np.float32(-np.inf)).astype(np.float64)
+    tiny = np.ldexp(row, -130)                                    # scale at its least, subnormal elements
+    huge = np.ldexp(row, 125)
+    x = np.stack([row, above, below, tiny, huge, np.zeros(32), np.full(32, 2.0 ** -149), np.full(32, -3.4028234e38)])
+    codes, scales = quantise(x.astype(np.float32).astype(np.float64))
+    q = ops.quantize_mx4(torch.from_numpy(x.astype(np.float32)).cuda())
+    got_codes, got_scales = rows_of(q)
+    assert np.array_equal(got_scales[:8, :1], scales)
+    assert np.array_equal(got_codes[:8, :32], codes)
+    assert np.array_equal(ops.dequantize_mx4(q, torch.float32).double().cpu().numpy(), values(codes, scales))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_quantize_not_finite(ops, bad, dtype):
+    """A block with an infinity or a NaN reads as NaN; its neighbours are untouched."""
+    x = normal((20, 200), 4, dtype=dtype)
+    x[3, 40] = x[19, 199] = bad
+    back = ops.dequantize_mx4(ops.quantize_mx4(x.cuda()), torch.float32).cpu()
+    want = values(*quantise(x.double().numpy()))
+    assert torch.isnan(back[3, 32:64]).all() and torch.isnan(back[19, 192:]).all()
+    assert int(torch.isnan(back).sum()) == 32 + 8
+    assert np.array_equal(back.double().numpy(), want, equal_nan=True)
+
+
+def test_quantising_again_changes_nothing(ops):
+    q = ops.quantize_mx4(normal((50, 700), 9, dtype=torch.bfloat16).cuda())
+    again = ops.quantize_mx4(ops.dequantize_mx4(q, torch.bfloat16))
+    assert torch.equal(q.codes, again.codes) and torch.equal(q.scales, again.scales)
+
+
+def test_quantize_rows_that_lie_apart(ops):
+    big = normal((37, 300), 5, dtype=torch.bfloat16).cuda()
+    for view in (big[:, :200], big[:, 3:190], big[::2, 64:128], big[5:6, 1:2]):
+        q, c = ops.quantize_mx4(view), ops.quantize_mx4(view.contiguous())
+        assert torch.equal(q.codes, c.codes) and torch.equal(q.scales, c.scales)
+
+
+@pytest.mark.parametrize("n,k", [(1, 1), (16, 32), (33, 63), (18, 160), (50, 1001)])
+def test_from_codes(ops, n, k):
+    rng = np.random.default_rng(n + k)
+    codes = rng.integers(0, 16, (n, k), dtype=np.uint8)
+    scales = rng.integers(100, 150, (n, -(-k // 32)), dtype=np.uint8)
+    scales[0, 0] = 255
+    packed, s = file_form(codes, scales)
+    padded = torch.full((n, packed.shape[1] + 5), 0xAB, dtype=torch.uint8)       # more columns than the rows need
+    padded[:, :packed.shape[1]] = packed
+    for held in (packed.cuda(), padded.cuda(), padded.cuda()[:, :packed.shape[1]]):
+        q = ops.mx4_from_codes(held, s.cuda(), k)
+        got_codes, got_scales = rows_of(q)
+        assert np.array_equal(got_codes[:n, :k], codes) and not got_codes[:, k:].any() and not got_codes[n:].any()
+        assert np.array_equal(got_scales[:n, :s.shape[1]], scales)
+        assert np.array_equal(ops.dequantize_mx4(q, torch.float32).double().cpu().numpy(), values(codes, scales),
+                              equal_nan=True)
+    if k % 2 == 0:
+        assert ops.mx4_from_codes(packed.cuda(), s.cuda()).shape == (n, k)
+
+
+# ------------------------------------------------------------------------------- products
+PRODUCTS = [(1, 16, 32), (1, 64, 2048), (2, 17, 40), (5, 100, 129), (16, 48, 1000), (17, 33, 256), (31, 80, 1023),
+            (33, 130, 512), (64, 96, 640), (65, 40, 1152), (100, 257, 384), (129, 64, 2000), (200, 300, 136),
+            (257, 520, 1024), (520, 272, 264)]
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_linear(ops, m, n, k, out):
+    x = normal((m, k), 7 * m + k, dtype=torch.bfloat16)
+    codes, scales, w = weight(n, k, n + k)
+    packed, s = file_form(codes, scales)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    got = ops.linear(x.cuda(), q, None, out)
+    assert got.dtype == out and got.shape == (m, n)
+    xd = x.double().numpy()
+    diff = np.abs(got.double().cpu().numpy() - xd @ w.T)
+    assert (diff <= bound(xd, w, k, out)).all(), (diff - bound(xd, w, k, out)).max()
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n,k", PRODUCTS)
+def test_linear_both_in_mxfp4(ops, m, n, k, out):
+    x = normal((m, k), 7 * m + k, dtype=torch.bfloat16)
+    codes, scales, w = weight(n, k, n + k)
+    packed, s = file_form(codes, scales)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    got = ops.linear(ops.quantize_mx4(x.cuda()), q, None, out)
+    assert got.dtype == out and got.shape == (m, n)
+    xd = values(*quantise(x.double().numpy()))
+    diff = np.abs(got.double().cpu().numpy() - xd @ w.T)
+    assert (diff <= bound(xd, w, k, out)).all(), (diff - bound(xd, w, k, out)).max()
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_linear_bias(ops, m, four):
+    n, k = 77, 224
+    x = normal((m, k), m, dtype=torch.bfloat16)
+    b = normal((n,), 3)
+    codes, scales, w = weight(n, k, 6)
+    packed, s = file_form(codes, scales)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    rows = ops.quantize_mx4(x.cuda()) if four else x.cuda()
+    xd = values(*quantise(x.double().numpy())) if four else x.double().numpy()
+    got = ops.linear(rows, q, b.cuda(), torch.float32).double().cpu().numpy()
+    # one more addition
+    lim = bound(xd, w, k, torch.float32) + 2 * HALF_F32 * (np.abs(xd @ w.T) + np.abs(b.double().numpy()))
+    assert (np.abs(got - (xd @ w.T + b.double().numpy())) <= lim).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh", "relu"])
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("m,inter,k", [(1, 16, 64), (3, 48, 200), (16, 33, 128), (20, 112, 600), (64, 80, 333),
+                                       (90, 17, 64), (150, 256, 512), (300, 144, 1024)])
+def test_gated(ops, m, inter, k, four, act):
+    x = normal((m, k), m + inter, dtype=torch.bfloat16)
+    codes, scales, w = weight(2 * inter, k, k + inter)
+    packed, s = file_form(codes, scales)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    rows = ops.quantize_mx4(x.cuda()) if four else x.cuda()
+    xd = values(*quantise(x.double().numpy())) if four else x.double().numpy()
+    got = ops.linear_swiglu(rows, q, torch.bfloat16, act)
+    assert got.dtype == torch.bfloat16 and got.shape == (m, inter)
+    y = xd @ w.T
+    g, u = y[:, :inter], y[:, inter:]
+    want = gate(act, g, u)
+    # gate and up are off by what a float32 sum may be (dg, du); |act'| <= 1.2 and |act(g)| <= |g|, the
+    # activation itself within 2^-16 of |g| (exp and tanh of the device, the cancellation in 1 + tanh
+    # near -1), then one rounding of the result
+    d = bound(xd, w, k, torch.float32)
+    dg, du = d[:, :inter], d[:, inter:]
+    lim = 1.2 * dg * (np.abs(u) + du) + (np.abs(g) + dg) * du + 2.0 ** -16 * np.abs(g) * np.abs(u)
+    lim = lim + HALF_BF16 * (np.abs(want) + lim) + 1e-38
+    assert (np.abs(got.double().cpu().numpy() - want) <= lim).all()
+
+
+def test_a_row_is_the_same_whatever_the_batch(ops):
+    x = normal((64, 1056), 8, dtype=torch.bfloat16).cuda()
+    q = ops.quantize_mx4(normal((208, 1056), 9, dtype=torch.bfloat16).cuda())
+    whole = ops.linear(x, q, None, torch.float32)
+    for m0, m in ((0, 1), (3, 7), (16, 16), (10, 33), (1, 63)):
+        assert torch.equal(ops.linear(x[m0:m0 + m], q, None, torch.float32), whole[m0:m0 + m])
+
+
+def test_rows_that_are_not_finite_stay_in_their_rows(ops):
+    k, n = 200, 48
+    x = normal((20, k), 8, dtype=torch.bfloat16)
+    x[4, 0], x[9, 199] = float("inf"), float("nan")
+    codes, scales, w = weight(n, k, 2)
+    packed, s = file_form(codes, scales)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    for rows in (x.cuda(), ops.quantize_mx4(x.cuda())):
+        got = ops.linear(rows, q, None, torch.float32).cpu()
+        assert torch.isfinite(got[[i for i in range(20) if i not in (4, 9)]]).all()
+        assert not torch.isfinite(got[4]).any() and torch.isnan(got[9]).all()
+
+
+def test_a_block_of_the_weight_that_is_nan(ops):
+    k, n = 160, 40
+    codes, scales, _ = weight(n, k, 2)
+    scales[7, 2] = 255
+    packed, s = file_form(codes, scales)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    x = normal((5, k), 8, dtype=torch.bfloat16).cuda()
+    for rows in (x, ops.quantize_mx4(x)):
+        got = ops.linear(rows, q, None, torch.float32).cpu()
+        assert torch.isnan(got[:, 7]).all() and int(torch.isnan(got).sum()) == 5
+
+
+def test_rows_that_lie_apart_or_askew(ops):
+    big = normal((40, 300), 5, dtype=torch.bfloat16).cuda()
+    q = ops.quantize_mx4(normal((70, 130), 6).cuda())
+    for view in (big[:, :130], big[:, 1:131], big[::3, 8:138], big[:1, 5:135]):
+        assert torch.equal(ops.linear(view, q, None, torch.float32), ops.linear(view.contiguous(), q, None, torch.float32))
+
+
+def test_no_rows(ops):
+    q = ops.quantize_mx4(normal((32, 64), 1).cuda())
+    none = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda")
+    assert ops.linear(none, q, None, torch.bfloat16).shape == (0, 32)
+    assert ops.linear_swiglu(none, q).shape == (0, 16)
+
+
+def test_leading_rows(ops):
+    w = normal((64, 200), 1).cuda()
+    q = ops.quantize_mx4(w)
+    x = normal((5, 200), 2, dtype=torch.bfloat16).cuda()
+    assert torch.equal(ops.linear(x, q.leading_rows(32), None, torch.float32), ops.linear(x, q, None, torch.float32)[:, :32])
+    with pytest.raises(KernelError):
+        q.leading_rows(20)
+    with pytest.raises(KernelError):
+        q.leading_rows(80)
+
+
+def test_refusals(ops):
+    w = normal((32, 64), 1).cuda()
+    q = ops.quantize_mx4(w)
+    x = normal((4, 64), 2, dtype=torch.bfloat16).cuda()
+    codes = torch.zeros((4, 16), dtype=torch.uint8, device="cuda")
+    scales = torch.zeros((4, 1), dtype=torch.uint8, device="cuda")
+    bad = [
+        lambda: ops.quantize_mx4(w.half()),
+        lambda: ops.quantize_mx4(w.t()),
+        lambda: ops.quantize_mx4(w[0]),
+        lambda: ops.quantize_mx4(w.cpu()),
+        lambda: ops.quantize_mx4(w[:0]),
+        lambda: ops.quantize_mx4(w[:, :0]),
+        lambda: ops.dequantize_mx4(q, torch.float16),
+        lambda: ops.dequantize_mx4(w, torch.float32),
+        lambda: ops.mx4_from_codes(codes.int(), scales),
+        lambda: ops.mx4_from_codes(codes, scales.float()),
+        lambda: ops.mx4_from_codes(codes, scales, 33),
+        lambda: ops.mx4_from_codes(codes, scales, 0),
+        lambda: ops.mx4_from_codes(codes, scales[:3]),
+        lambda: ops.mx4_from_codes(codes.cpu(), scales),
+        lambda: ops.linear(x.float(), q, None, torch.float32),
+        lambda: ops.linear(x[:, :32], q, None, torch.float32),
+        lambda: ops.linear(x.t().contiguous().t(), q, None, torch.float32),
+        lambda: ops.linear(x.cpu(), q, None, torch.float32),
+        lambda: ops.linear(x, q, None, torch.float16),
+        lambda: ops.linear(x, q, torch.zeros(31, device="cuda"), torch.float32),
+        lambda: ops.linear(ops.quantize_mx4(x), w.bfloat16(), None, torch.float32),
+        lambda: ops.linear_swiglu(ops.quantize_mx4(x), w.bfloat16()),
+        lambda: ops.linear_swiglu(x, ops.quantize_mx4(w[:31])),
+        lambda: ops.linear_swiglu(x, q, torch.bfloat16, "tanh"),
+        lambda: ops.linear_swiglu(x[:, :32], q),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(KernelError):
+            call()
+            pytest.fail("call %d was not refused" % i)
+
+
+def test_quantise_and_multiply_replayed_from_a_graph(ops):
+    """A run as a step makes it (rows rounded, gated product, product) captured once and replayed
+    over new rows, with eager work between the replays."""
+    gate_up = ops.quantize_mx4(normal((2 * 96, 128), 1, 0.1).cuda())
+    down = ops.quantize_mx4(normal((128, 96), 2, 0.1).cuda())
+    x = torch.empty((24, 128), dtype=torch.bfloat16, device="cuda")
+    held = {}
+
+    def step():
+        h = ops.linear_swiglu(x, gate_up)
+        held["out"] = ops.linear(ops.quantize_mx4(h), down, None, torch.bfloat16)
+    x.normal_()
+    graph = ops.capture(step)
+    replayed = held["out"]
+    for i in range(4):
+        x.copy_(normal((24, 128), 50 + i))
+        graph.replay()
+        got = replayed.clone()
+        step()
+        assert torch.equal(got, held["out"])
+        torch.cuda.synchronize()
+
+
+def test_on_another_stream(ops):
+    w, x = normal((64, 256), 1).cuda(), normal((3, 256), 2, dtype=torch.bfloat16).cuda()
+    want = ops.linear(x, ops.quantize_mx4(w), None, torch.float32)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = ops.linear(x, ops.quantize_mx4(w), None, torch.float32)
+    side.synchronize()
+    assert torch.equal(got, want)
