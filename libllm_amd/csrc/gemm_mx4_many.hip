@@ -1,0 +1,475 @@
+// C[M,N] = X[M,K] * W[N,K]^T for a weight in MXFP4 (mx4.h) and many rows, bound by the matrix cores
+// and by what a compute unit can pull into its shared memory.  Rows in bfloat16: W's codes are widened
+// to bfloat16 in front of v_mfma_f32_16x16x32_bf16, exactly, so the result is that of a bfloat16
+// product with W's numbers.  Rows in MXFP4: v_mfma_scale_f32_16x16x128_f8f6f4, four times the
+// arithmetic an instruction.  Sums in float32; result bfloat16 or float32, or gated over a stacked
+// [gate; up] weight (out[m, i] = act(gate_i) * up_i, in 32 bits until the one rounding).
+//
+// A block of waves, WM along the rows of X by WN along those of W, owns 16 WM MTW rows of X by
+// 16 WN NTW rows of W (gated: half of them gate, half the up rows of the same columns); W is the A
+// operand, so that a lane ends with four consecutive columns of one row of C.  K goes by in tiles:
+// 128 elements (bfloat16, four steps of 32) or 256 (MXFP4, two steps of 128).  X's tiles go from
+// memory straight into LDS (global_load_lds_dwordx4), two buffers.  In bfloat16 a row of a tile is 256
+// bytes in 16 pieces; piece p of row r lies at p ^ (r & 15), so that the 16 rows a fragment read
+// touches fall into different banks.  In MXFP4 the tiles lie in lane order as they come.  W's codes
+// are a quarter of X's bytes: with rows in bfloat16 they stay in registers, read straight from the
+// caches by every wave that needs them, one tile of K ahead; with rows in MXFP4 they go through LDS
+// like X's, and the scales too, four units at a time.
+//
+// The fragments of a step are read into registers one step ahead of the matrix instructions that use
+// them, dealt out between those; the barrier of a tile lies in front of its last step, whose
+// fragments every wave has by then: behind it the loads of the tile after next go out into the
+// buffer that is left, and the first fragments of the next tile are read.
+#include "mx4.h"
+
+#include <type_traits>
+
+#define MM_EPI_NONE 0
+#define MM_EPI_GATED 1
+
+struct Mx4ManyArgs {
+  const bf16_t* X;           // rows in bfloat16, ldx apart; K and ldx multiples of 128
+  const uint8_t* xc;         // or rows in MXFP4
+  const uint8_t* xs;
+  const uint8_t* wc;
+  const uint8_t* ws;
+  const float* bias;         // [N] or null (plain epilogue)
+  void* C;
+  int M, N, n_out;
+  int ldx, units, quads, act;
+  int m_tiles, n_tiles;      // blocks along X and W
+  hipStream_t stream;
+};
+
+template <int N, typename F> __device__ __forceinline__ void each(F&& f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
+
+// 16 bytes a lane from base + off into LDS, in lane order from `lds` on, without registers in
+// between.  Written in assembly: the compiler would make every read of LDS wait for all of them (it
+// cannot tell that they fill the other buffer).  It does not count them either: the kernel waits
+// for them itself, before the barrier that hands a buffer over.  (The instruction takes its place in
+// LDS from M0, which is put back: the compiler need not know.)
+__device__ __forceinline__ void lds_fill(uint32_t lds, const void* base, uint32_t off) {
+  uint32_t m0_was;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+               : "=&s"(m0_was) : "s"(lds), "v"(off), "s"(base) : "memory");
+}
+
+template <bool X4, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
+__global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  constexpr int NW = WM * WN;
+  constexpr int BM = WM * MTW * 16, BNT = WN * NTW;         // rows of X, tiles of W a block
+  constexpr int STEPS = X4 ? 2 : 4;
+  constexpr int XB = X4 ? BM * 128 : BM * 256;              // bytes of X's tile of K
+  constexpr int WB = X4 ? BNT * 2048 : 0;                   // of W's, where it goes through LDS
+  constexpr int BUF = XB + WB;
+  constexpr int TILES = BM / 16 + BNT;
+  constexpr int SB = X4 ? TILES * 256 : 0;                  // scales of a quad: W's tiles, then X's
+  constexpr int FILLS = BUF / 1024 / NW;                    // 1 KiB each
+  static_assert(BUF % (1024 * NW) == 0, "every wave fills as much");
+  constexpr bool GATED = EPI == MM_EPI_GATED;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int wm = wave % WM, wn = wave / WM;
+
+  // blocks i, i + 8, ... share a chiplet: a chiplet takes every eighth tile of W rows and, at a
+  // time, a band of 8 tiles of X rows
+  const int xcd = blockIdx.x & 7, jb = blockIdx.x >> 3;
+  const int n_per = (a.n_tiles + 7) >> 3;
+  const int band = jb / (8 * n_per), jj = jb - band * (8 * n_per);
+  const int band_rows = min(a.m_tiles - band * 8, 8);
+  const int mt_blk = band * 8 + jj % band_rows, nt_blk = (jj / band_rows) * 8 + xcd;
+  if (nt_blk >= a.n_tiles || jj >= band_rows * n_per) return;
+  const int m0 = mt_blk * BM;
+  const int out_tiles = (a.n_out + 15) / 16;
+
+  // tile of W that is number t of this block (past the end the last one; its sums are not stored)
+  auto w_tile = [&](int t) {
+    if (GATED) return min(nt_blk * (BNT / 2) + t % (BNT / 2), out_tiles - 1) + (t / (BNT / 2)) * out_tiles;
+    return min(nt_blk * BNT + t, out_tiles - 1);
+  };
+  // number within the block of tile nt of this wave: gated, its gate tiles and then its up tiles
+  auto wave_tile = [&](int nt) {
+    return GATED ? (nt / (NTW / 2)) * (BNT / 2) + wn * (NTW / 2) + nt % (NTW / 2) : wn * NTW + nt;
+  };
+  const size_t c_tile = (size_t)a.quads * 4096, s_tile = (size_t)a.quads * 256;
+
+  // ---- what this wave fills, and where from
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
+  static_assert(X4 || NW % 4 == 0, "the rows a wave fills lie a multiple of 16 apart");
+  const uint32_t lane16 = lane * 16, lane4 = lane * 4;
+  const uint8_t* fill_base[X4 ? FILLS : 1];
+  int fill_row = 0;
+  uint32_t fill_piece = 0;
+  if constexpr (X4) {
+#pragma unroll
+    for (int p = 0; p < FILLS; ++p) {
+      const int c = p * NW + wave, t = c >> 1;              // which KiB of the buffer: (tile, unit) of X, then of W
+      fill_base[p] = (t < BM / 16 ? a.xc + (size_t)min(m0 / 16 + t, (a.M - 1) / 16) * c_tile
+                                  : a.wc + (size_t)w_tile(t - BM / 16) * c_tile) + (c & 1) * 1024;
+    }
+  } else {                                                  // four rows of X
+    fill_base[0] = (const uint8_t*)(a.X + (size_t)m0 * a.ldx);
+    fill_row = wave * 4 + g;
+    fill_piece = (r ^ (fill_row & 15)) * 16;
+  }
+  // scales of a quad: a KiB is four tiles; waves beyond them fill what another wave fills, with the same
+  constexpr int SC_WAVES = TILES / 4;
+  static_assert(!X4 || (TILES % 4 == 0 && SC_WAVES <= NW), "a wave fills the scales of four tiles at most");
+  const int sc_wave = X4 ? wave % SC_WAVES : 0;
+  const uint8_t* sc_base = nullptr;
+  if constexpr (X4) {
+    const int t = sc_wave * 4 + (lane >> 4);
+    sc_base = (t < BNT ? a.ws + (size_t)w_tile(t) * s_tile
+                       : a.xs + (size_t)min(m0 / 16 + t - BNT, (a.M - 1) / 16) * s_tile) + (lane & 15) * 16;
+  }
+  const int n_kt = X4 ? (a.units + 1) / 2 : a.units;
+  // Tile kt of K into buffer `buf`; past the last tile the last one again, which nobody reads: the
+  // loop has no branch then, over which the compiler would move matrix instructions.
+  auto fill = [&](int kt, int buf, int p) {
+    const uint32_t at = lds0 + buf * BUF + (p * NW + wave) * 1024;
+    if constexpr (X4) {
+      lds_fill(at, fill_base[p] + (size_t)min(kt, n_kt - 1) * 2048, lane16);
+    } else {                                                // (the offset made anew each time: held, it would cost a register a fill)
+      int row = fill_row;
+      asm volatile("" : "+v"(row));
+      row = min(row + p * NW * 4, a.M - 1 - m0);
+      lds_fill(at, fill_base[0] + (size_t)min(kt, n_kt - 1) * 256, (uint32_t)row * (uint32_t)a.ldx * 2 + fill_piece);
+    }
+  };
+  auto fill_scales = [&](int q, int buf) {
+    if constexpr (X4) {
+      uint32_t m0_was;
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
+                   : "=&s"(m0_was) : "s"(lds0 + 2 * BUF + buf * SB + sc_wave * 1024),
+                     "v"(sc_base + (size_t)min(q, a.quads - 1) * 256) : "memory");
+    }
+  };
+
+  f32x4 acc[NTW][MTW];
+#pragma unroll
+  for (int nt = 0; nt < NTW; ++nt)
+#pragma unroll
+    for (int mt = 0; mt < MTW; ++mt) acc[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // ---- fragments.  The matrix instructions of a step go by row tile of X: once a tile's are issued,
+  // its fragment of the next step is read into the same registers.  Addresses are kept few: the
+  // compiler would hold one for every read of the loop and run out of registers.
+  typedef uint32_t u4_raw __attribute__((ext_vector_type(4)));
+  Frag xf[MTW];
+  Frag wf[2][X4 ? NTW : 1];
+  uint32_t sc[2][X4 ? (NTW + MTW) / 2 : 1];                 // scales of a tile of K: two bytes of two tiles a word
+  u4_raw wc[2][X4 ? 1 : NTW];                               // W's codes of a tile of K, and its scales
+  uint32_t wsc[2][X4 ? 1 : NTW];
+  const uint32_t x_lane = lds0 + wm * MTW * (X4 ? 2048 : 4096) + (X4 ? lane16 : r * 256 + ((g * 4) ^ r) * 16);
+  const uint32_t w_lane = lds0 + XB + lane16;
+  typedef const __attribute__((address_space(3))) u4_raw* lds_u4;
+  typedef const __attribute__((address_space(3))) uint16_t* lds_u2;
+  typedef const __attribute__((address_space(1))) u4_raw* global_u4;
+  typedef const __attribute__((address_space(1))) uint32_t* global_u1;
+  auto plus = [&](uint32_t lane_at, int by) {
+    uint32_t at;
+    asm volatile("v_add_u32 %0, %1, %2" : "=v"(at) : "s"(by), "v"(lane_at));
+    return at;
+  };
+  auto x_step = [&](int buf, int step) {                    // (piece 4 g + step of row r lies at its xor with r)
+    uint32_t at = x_lane;
+    if constexpr (!X4) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(at) : "s"(step * 16), "v"(x_lane));
+    return plus(at, buf * BUF + (X4 ? step * 1024 : 0));
+  };
+  auto lds_read = [&](uint32_t at) {
+    const u4_raw v = *(lds_u4)(uintptr_t)at;
+    Frag f;
+    f.u = make_uint4(v.x, v.y, v.z, v.w);
+    return f;
+  };
+  auto read_x = [&](uint32_t at, int mt) { return lds_read(at + mt * (X4 ? 2048 : 4096)); };
+  auto read_w = [&](uint32_t at, int nt) { return lds_read(at + wave_tile(nt) * 2048); };
+  auto read_scales = [&](uint32_t at, int i, uint32_t& lo, uint32_t& hi) {      // word i: tiles 2 i and 2 i + 1, W's first
+    const int t0 = 2 * i < NTW ? wave_tile(2 * i) : BNT + wm * MTW + 2 * i - NTW;
+    const int t1 = 2 * i < NTW ? wave_tile(2 * i + 1) : t0 + 1;
+    lo = *(lds_u2)(uintptr_t)(at + t0 * 256);
+    hi = *(lds_u2)(uintptr_t)(at + t1 * 256);
+  };
+  auto load_w = [&](int kt, int set) {
+#pragma unroll
+    for (int nt = 0; nt < NTW; ++nt) {
+      const size_t t = w_tile(wave_tile(nt));
+      const uint8_t* codes = a.wc + t * c_tile + (size_t)kt * 1024;
+      const uint8_t* scales = a.ws + t * s_tile + (size_t)(kt >> 2) * 256;
+      asm volatile("" : "+s"(codes), "+s"(scales));
+      wc[set][nt] = *(global_u4)(codes + lane16);
+      wsc[set][nt] = *(global_u1)(scales + lane4);
+    }
+  };
+
+  each<FILLS>([&](auto p) { fill(0, 0, p); });
+  fill_scales(0, 0);
+  each<FILLS>([&](auto p) { fill(1, 1, p); });
+  // (the compiler is told that it has W's codes: else it would wait for them, and with them for every
+  // load into LDS behind them, inside the loop)
+  auto have_w = [&](int set) {
+#pragma unroll
+    for (int nt = 0; nt < NTW; ++nt) asm volatile("" : "+v"(wc[set][nt]), "+v"(wsc[set][nt]));
+  };
+  if constexpr (!X4) {
+    load_w(0, 0);
+    have_w(0);
+  }
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // everything this wave asked for has arrived
+  __syncthreads();
+  {
+    const uint32_t x_at = x_step(0, 0);
+#pragma unroll
+    for (int mt = 0; mt < MTW; ++mt) xf[mt] = read_x(x_at, mt);
+  }
+  if constexpr (X4) {
+#pragma unroll
+    for (int nt = 0; nt < NTW; ++nt) wf[0][nt] = read_w(w_lane, nt);
+#pragma unroll
+    for (int i = 0; i < (NTW + MTW) / 2; ++i) {
+      uint32_t lo, hi;
+      read_scales(lds0 + 2 * BUF + lane4, i, lo, hi);
+      sc[0][i] = lo | hi << 16;
+    }
+  }
+
+  // one tile of K; CUR: which set of scales (or codes of W) is its own, and the buffer it lies in
+  auto round = [&](int kt, auto cur) {
+    constexpr int CUR = decltype(cur)::value, NEXT = CUR ^ 1;
+    uint32_t sc_lo[(NTW + MTW) / 2], sc_hi[(NTW + MTW) / 2];
+    if constexpr (!X4) load_w(min(kt + 1, n_kt - 1), NEXT);
+    each<STEPS>([&](auto step) {
+      constexpr int S = decltype(step)::value, SET = S & 1;
+      constexpr bool LAST = S == STEPS - 1;
+      constexpr int RBUF = LAST ? NEXT : CUR, RS = LAST ? 0 : S + 1;      // where the next step's fragments lie
+      if constexpr (LAST) {
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!X4) have_w(NEXT);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __syncthreads();
+      }
+      const uint32_t x_at = x_step(RBUF, RS);
+      uint32_t w_at = 0, s_at = 0;
+      Frag w[X4 ? 1 : NTW];
+      if constexpr (X4) {
+        w_at = plus(w_lane, RBUF * BUF + RS * 1024);
+        if constexpr (LAST) s_at = plus(lane4, lds0 + 2 * BUF + (((kt + 1) >> 1) & 1) * SB + NEXT * 2);
+      } else {
+        const int sh = 8 * (kt & 3);
+#pragma unroll
+        for (int nt = 0; nt < NTW; ++nt) {
+          w[nt] = mx4_widen(wc[CUR][nt][S], mx4_scale((wsc[CUR][nt] >> sh) & 255u));
+        }
+      }
+      each<MTW>([&](auto mtc) {
+        constexpr int MT = decltype(mtc)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        // this group's share of the loads of the tile after next
+        if constexpr (LAST) {
+#pragma unroll
+          for (int p = FILLS * MT / MTW; p < FILLS * (MT + 1) / MTW; ++p) fill(kt + 2, CUR, p);
+          if (MT == 0 && CUR == 0) fill_scales((kt + 2) >> 1, ((kt + 2) >> 1) & 1);
+        }
+        each<NTW>([&](auto ntc) {
+          constexpr int NT = decltype(ntc)::value;
+          if constexpr (X4)
+            acc[NT][MT] = mx4_mfma<(NT & 1) * 2 + S, (MT & 1) * 2 + S>(wf[SET][NT].u, sc[CUR][NT / 2], xf[MT].u,
+                                                                       sc[CUR][NTW / 2 + MT / 2], acc[NT][MT]);
+          else
+            acc[NT][MT] = mfma_bf16(w[NT], xf[MT], acc[NT][MT]);
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        // its share of the next step's reads, behind them
+        xf[MT] = read_x(x_at, MT);
+        if constexpr (X4) {
+#pragma unroll
+          for (int nt = NTW * MT / MTW; nt < NTW * (MT + 1) / MTW; ++nt) wf[SET ^ 1][nt] = read_w(w_at, nt);
+          if constexpr (LAST) {
+            constexpr int NS = (NTW + MTW) / 2;
+#pragma unroll
+            for (int i = NS * MT / MTW; i < NS * (MT + 1) / MTW; ++i) read_scales(s_at, i, sc_lo[i], sc_hi[i]);
+          }
+        }
+      });
+    });
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (X4) {
+#pragma unroll
+      for (int i = 0; i < (NTW + MTW) / 2; ++i) sc[NEXT][i] = sc_lo[i] | sc_hi[i] << 16;
+    }
+  };
+  static_assert(STEPS % 2 == 0, "a tile of K ends on the set of W's fragments that it began with");
+  int kt = 0;
+  for (; kt + 2 <= n_kt; kt += 2) {
+    round(kt, std::integral_constant<int, 0>{});
+    round(kt + 1, std::integral_constant<int, 1>{});
+  }
+  if (kt < n_kt) round(kt, std::integral_constant<int, 0>{});
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // the last loads into LDS have landed too
+
+  // ---- epilogue: lane holds C[m = .. + r][n = .. + 4 g + e]
+  constexpr int OUT_NT = GATED ? NTW / 2 : NTW;
+  const int n_wave = (nt_blk * (GATED ? BNT / 2 : BNT) + wn * OUT_NT) * 16, m_wave = m0 + wm * MTW * 16;
+  float bias[OUT_NT][4];
+#pragma unroll
+  for (int nt = 0; nt < OUT_NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int n = n_wave + nt * 16 + 4 * g + e;
+      bias[nt][e] = !GATED && a.bias != nullptr && n < a.n_out ? a.bias[n] : 0.f;
+    }
+  auto value = [&](int nt, int mt, float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = acc[nt][mt][e];
+      if (GATED) {
+        const float gt = acc[nt][mt][e], up = acc[nt + NTW / 2 < NTW ? nt + NTW / 2 : nt][mt][e];
+        v[e] = a.act == LLM_ACT_SILU ? up * gt * __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.4426950408889634f * gt))
+                                     : llm_gated(a.act, gt, up);
+      } else {
+        v[e] += bias[nt][e];
+      }
+    }
+  };
+  if constexpr (sizeof(OutT) == 4) {                        // 64 bytes of a row in a store: whole pieces of lines
+#pragma unroll
+    for (int nt = 0; nt < OUT_NT; ++nt)
+#pragma unroll
+      for (int mt = 0; mt < MTW; ++mt) {
+        const int m = m_wave + mt * 16 + r, n = n_wave + nt * 16 + 4 * g;
+        if (m >= a.M || n >= a.n_out) continue;
+        float v[4];
+        value(nt, mt, v);
+        float* dst = (float*)a.C + (size_t)m * a.n_out + n;
+        if (n + 3 < a.n_out && (a.n_out & 3) == 0) {
+          *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n + e < a.n_out) dst[e] = v[e];
+        }
+      }
+  } else {
+    // Each wave turns its tile round through a region of LDS of its own, 16 rows of X at a time, rows 16
+    // bytes longer than they are so that the 16 rows of a write fall into different banks, and then
+    // stores whole rows, 16 bytes a lane.
+    __syncthreads();                                        // every wave has read the last tile
+    constexpr int COLS = OUT_NT * 16, ROW_B = COLS * 2 + 16;
+    constexpr int LPR = COLS / 8, RPP = 64 / LPR;           // lanes a row, rows a store
+    unsigned char* mine = lds + wave * (16 * ROW_B);
+    const int col = (lane % LPR) * 8;
+#pragma unroll
+    for (int mt = 0; mt < MTW; ++mt) {
+#pragma unroll
+      for (int nt = 0; nt < OUT_NT; ++nt) {
+        float v[4];
+        value(nt, mt, v);
+        uint2 pk;
+        pk.x = pack2_bf16(v[0], v[1]);
+        pk.y = pack2_bf16(v[2], v[3]);
+        *reinterpret_cast<uint2*>(mine + r * ROW_B + (nt * 16 + 4 * g) * 2) = pk;
+      }
+      // (a wave's accesses to LDS run in order; the compiler may not move one lane's read over another's write)
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int pass = 0; pass < (16 + RPP - 1) / RPP; ++pass) {
+        const int row = pass * RPP + lane / LPR;
+        const int m = m_wave + mt * 16 + row, n = n_wave + col;
+        if (row < 16 && m < a.M && n < a.n_out) {
+          const uint4 v = *reinterpret_cast<const uint4*>(mine + row * ROW_B + col * 2);
+          bf16_t* dst = (bf16_t*)a.C + (size_t)m * a.n_out + n;
+          if (n + 7 < a.n_out && (a.n_out & 7) == 0) {
+            *reinterpret_cast<uint4*>(dst) = v;
+          } else {
+            const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < a.n_out) dst[e] = (bf16_t)(w4[e >> 1] >> (16 * (e & 1)));
+          }
+        }
+      }
+      asm volatile("" ::: "memory");
+    }
+  }
+}
+
+template <bool X4, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
+static int launch_mx4_many(Mx4ManyArgs a) {
+  constexpr int BM = WM * MTW * 16, BNT = WN * NTW, NW = WM * WN;
+  constexpr int BUF = X4 ? BM * 128 + BNT * 2048 : BM * 256, SB = X4 ? (BM / 16 + BNT) * 256 : 0;
+  constexpr int OUT_NT = EPI == MM_EPI_GATED ? NTW / 2 : NTW;
+  constexpr int TURN = NW * 16 * (OUT_NT * 32 + 16);
+  constexpr int LDS_BYTES = 2 * (BUF + SB) > TURN ? 2 * (BUF + SB) : TURN;
+  static_assert(LDS_BYTES <= 160 * 1024, "shared memory of a unit");
+  const int out_tiles = (a.n_out + 15) / 16, per = EPI == MM_EPI_GATED ? BNT / 2 : BNT;
+  a.m_tiles = (a.M + BM - 1) / BM;
+  a.n_tiles = (out_tiles + per - 1) / per;
+  const long long blocks = 8LL * ((a.m_tiles + 7) / 8) * 8 * ((a.n_tiles + 7) / 8);   // surplus blocks leave at once
+  if (blocks > 0x7fffffffLL) return LLM_ERR_ARG;
+  // more than 64 KiB of LDS has to be asked for, once per device and kernel
+  static bool asked[64];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return LLM_ERR_LAUNCH;
+  if (!asked[dev]) {
+    if (hipFuncSetAttribute((const void*)gemm_mx4_many_kernel<X4, WM, WN, MTW, NTW, EPI, OutT>,
+                            hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES) != hipSuccess)
+      return LLM_ERR_LAUNCH;
+    asked[dev] = true;
+  }
+  gemm_mx4_many_kernel<X4, WM, WN, MTW, NTW, EPI, OutT><<<(unsigned)blocks, NW * 64, LDS_BYTES, a.stream>>>(a);
+  return llm_launch_status();
+}
+
+template <bool X4, int EPI, typename OutT>
+static int pick_mx4_many(const Mx4ManyArgs& a) {
+  return launch_mx4_many<X4, 2, 4, 8, 4, EPI, OutT>(a);
+}
+
+template <bool X4>
+static int mx4_many(const Mx4ManyArgs& a, int epilogue, int out_dtype) {
+  if (epilogue == MM_EPI_GATED) return out_dtype == LLM_DTYPE_BF16 ? pick_mx4_many<X4, MM_EPI_GATED, bf16_t>(a) : LLM_ERR_ARG;
+  if (out_dtype == LLM_DTYPE_BF16) return pick_mx4_many<X4, MM_EPI_NONE, bf16_t>(a);
+  if (out_dtype == LLM_DTYPE_F32) return pick_mx4_many<X4, MM_EPI_NONE, float>(a);
+  return LLM_ERR_ARG;
+}
+
+// W [N, K] as mx4.h lays it out.  X: bfloat16 rows ldx apart with xs null (their length K and ldx
+// multiples of 128, what lies beyond W's width zero), or codes with their scales in xs.  epilogue 0:
+// C [M, N] of out_dtype, plus bias[n] if not null; 1 | act << 4: C [M, N / 2] in bfloat16, the gate
+// through an activation of common.h, N / 2 a multiple of 16.
+extern "C" int llm_gemm_mx4_many(const void* X, const void* xs, int ldx, const void* wc, const void* ws,
+                                 const float* bias, void* C, int epilogue, int out_dtype, int M, int N, int K,
+                                 hipStream_t stream) {
+  if (M <= 0) return LLM_OK;
+  const int act = epilogue >> 4;
+  epilogue &= 15;
+  if (epilogue != MM_EPI_NONE && epilogue != MM_EPI_GATED) return LLM_ERR_ARG;
+  if (N <= 0 || K <= 0 || act < 0 || act >= LLM_ACT_COUNT || (epilogue != MM_EPI_GATED && act != 0)) return LLM_ERR_ARG;
+  if (X == nullptr || wc == nullptr || ws == nullptr || C == nullptr) return LLM_ERR_ARG;
+  if ((((uintptr_t)X) | ((uintptr_t)wc) | ((uintptr_t)ws) | ((uintptr_t)C) | ((uintptr_t)xs)) & 15) return LLM_ERR_ARG;
+  if (xs == nullptr && (ldx < K || (ldx & 127) || (K & 127) || ldx > (1 << 22))) return LLM_ERR_ARG;   // (offsets within a block's rows stay below 2^32)
+  if (epilogue == MM_EPI_GATED && ((N & 31) || bias != nullptr)) return LLM_ERR_ARG;
+  Mx4ManyArgs a{};
+  a.X = (const bf16_t*)X;
+  a.xc = (const uint8_t*)X;
+  a.xs = (const uint8_t*)xs;
+  a.wc = (const uint8_t*)wc;
+  a.ws = (const uint8_t*)ws;
+  a.bias = bias;
+  a.C = C;
+  a.M = M;
+  a.N = N;
+  a.n_out = epilogue == MM_EPI_GATED ? N / 2 : N;
+  a.ldx = ldx;
+  a.units = mx4_units(K);
+  a.quads = mx4_quads(K);
+  a.act = act;
+  a.stream = stream;
+  return xs == nullptr ? mx4_many<false>(a, epilogue, out_dtype) : mx4_many<true>(a, epilogue, out_dtype);
+}

@@ -5,13 +5,16 @@
 // (out[m, i] = act(gate_i) * up_i, both still in 32 bits: one rounding).
 //
 // The waves of a block split K, a run of units of 128 elements each, and every wave goes through its
-// run alone: W and X go from memory straight into registers, STAGES units ahead of the arithmetic,
-// with no shared memory and no barrier until the waves' sums are added there, in their order.  The
-// waves of a block read different elements of X, so sharing them would gain nothing.  Which wave
-// adds which unit does not depend on M: an output is the same bits whatever else is in the batch.
+// run alone, with no barrier until the waves' sums are added at the end, in their order.  W goes from
+// memory straight into registers, STAGES units ahead of the arithmetic.  Rows of X in bfloat16 are
+// loaded as they lie, four rows by 256 bytes an instruction (whole lines), also STAGES ahead, and
+// turned into the matrix cores' operand through 4 KiB of shared memory that only this wave uses;
+// read straight from memory in operand order, 16 rows by four pieces of 16 bytes far apart, they
+// bounded the kernel (8 rows, K 14,336, 4,096 outputs: 18.0 us).  The waves of a block read
+// different elements of X, so sharing them would gain nothing.  Which wave adds which unit does not
+// depend on M: an output is the same bits whatever else is in the batch.
 #include "mx4.h"
 
-#define MR_WAVES 8           // waves that split K
 #define MR_EPI_NONE 0
 #define MR_EPI_GATED 1
 
@@ -25,24 +28,25 @@ struct Mx4Args {
   void* C;
   int M, N, K;               // N: rows of W
   int n_out;                 // columns of C: N, or N / 2 if gated
-  int ldx, units, quads, act;
+  int ldx, units, quads, act;   // units: those that hold elements of K
   hipStream_t stream;
 };
 
-// Rows of X of a unit, as lane l's B operands.
-template <int MT, bool X4> struct RowsOf;
-template <int MT> struct RowsOf<MT, false> { Frag f[MT][4]; };
-template <int MT> struct RowsOf<MT, true> { uint4 c[MT]; uint32_t s[MT]; };
-
-template <int MT, int RT, int STAGES, int EPI, typename OutT, bool X4>
-__global__ __launch_bounds__(MR_WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
+// WAVES: waves that split K; MT: tiles of 16 rows of X; XQ: quarters of a tile of which rows exist (4 unless MT is 1);
+// RT: tiles of W a wave; STAGES: units in flight.
+template <int WAVES, int MT, int XQ, int RT, int STAGES, int EPI, typename OutT, bool X4>
+__global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
   constexpr int RPR = EPI == MR_EPI_GATED ? 2 : 1;        // tiles of W that make one tile of outputs
   constexpr int OUT_RT = RT / RPR;
-  __shared__ __attribute__((aligned(16))) float red[MR_WAVES * RPR * MT * 256];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
+  constexpr int XL = X4 ? MT : (MT - 1) * 4 + XQ;         // loads of rows of X a unit
+  constexpr int WAVE_B = X4 ? RPR * MT * 1024 : 4096 * MT;
+  __shared__ __attribute__((aligned(16))) unsigned char lds[WAVES * WAVE_B];
+  float* red = reinterpret_cast<float*>(lds);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
   const int out_tile0 = blockIdx.x * OUT_RT, m0 = blockIdx.y * (16 * MT);
   const int out_tiles = (a.n_out + 15) / 16;
+  unsigned char* mine = lds + wave * WAVE_B;
 
   const uint4* wc[RT];
   const uint32_t* ws[RT];
@@ -51,24 +55,25 @@ __global__ __launch_bounds__(MR_WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a)
     int t = out_tile0 + rt / RPR;
     if (t > out_tiles - 1) t = out_tiles - 1;             // (not stored)
     if (RPR == 2) t += (rt & 1) * out_tiles;              // up follows gate; n_out is a multiple of 16
-    wc[rt] = a.wc + (size_t)t * a.units * 64 + lane;
+    wc[rt] = a.wc + (size_t)t * a.quads * 256 + lane;
     ws[rt] = a.ws + (size_t)t * a.quads * 64 + lane;
   }
-  const bf16_t* xp[MT];
-  bool x_on[MT];
-  size_t xt[MT];
+  // Rows past the end are read as the last row (bfloat16) or tile (MXFP4); their sums are not stored.
+  const bf16_t* xp[XL];
+  const uint4* xc[MT];
+  const uint32_t* xs[MT];
+#pragma unroll
+  for (int i = 0; i < XL; ++i) xp[i] = a.X + (size_t)min(m0 + i * 4 + g, a.M - 1) * a.ldx;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
-    const int row = m0 + mt * 16 + r;
-    x_on[mt] = X4 ? m0 + mt * 16 < a.M : row < a.M;
-    xp[mt] = a.X + (size_t)(row < a.M ? row : 0) * a.ldx + g * MX4_BLOCK;
-    xt[mt] = (size_t)(m0 / 16 + mt);
+    const size_t t = min(m0 / 16 + mt, (a.M - 1) / 16);
+    xc[mt] = a.xc + t * a.quads * 256 + lane;
+    xs[mt] = a.xs + t * a.quads * 64 + lane;
   }
 
   struct Stage {
-    uint4 w[RT];
-    uint32_t s[RT];
-    RowsOf<MT, X4> x;
+    uint4 w[RT], x[XL];
+    uint32_t s[RT], xs[X4 ? MT : 1];
   };
   auto load = [&](int u, Stage& st) {
 #pragma unroll
@@ -77,17 +82,17 @@ __global__ __launch_bounds__(MR_WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a)
       st.w[rt] = make_uint4(v.x, v.y, v.z, v.w);
       st.s[rt] = ws[rt][(size_t)(u >> 2) * 64];
     }
+    if constexpr (X4) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      if constexpr (X4) {
-        st.x.c[mt] = x_on[mt] ? a.xc[(xt[mt] * a.units + u) * 64 + lane] : make_uint4(0u, 0u, 0u, 0u);
-        st.x.s[mt] = x_on[mt] ? a.xs[(xt[mt] * a.quads + (u >> 2)) * 64 + lane] : 0u;
-      } else {
-        const int k = u * MX4_UNIT + g * MX4_BLOCK;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          st.x.f[mt][j] = (x_on[mt] && k + 8 * j < a.K) ? frag_load(xp[mt] + (size_t)u * MX4_UNIT + 8 * j) : frag_zero();
+      for (int mt = 0; mt < MT; ++mt) {
+        st.x[mt] = xc[mt][(size_t)u * 64];
+        st.xs[mt] = xs[mt][(size_t)(u >> 2) * 64];
       }
+    } else {
+      const int k = u * MX4_UNIT + r * 8;                 // piece r of a row's 256 bytes
+      const int at = k < a.K ? k : 0;
+#pragma unroll
+      for (int i = 0; i < XL; ++i) st.x[i] = *reinterpret_cast<const uint4*>(xp[i] + at);
     }
   };
   f32x4 acc[RT][MT];
@@ -95,30 +100,54 @@ __global__ __launch_bounds__(MR_WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a)
   for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) acc[rt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](int u, const Stage& st) {
+  auto compute = [&](int u, Stage& st) {
     const int sh = 8 * (u & 3);
+    if constexpr (X4) {
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if constexpr (X4) {
-        const uint32_t sa = st.s[rt] >> sh;
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
-          acc[rt][mt] = mx4_mfma<0, 0>(st.w[rt], sa, st.x.c[mt], st.x.s[mt] >> sh, acc[rt][mt]);
-      } else {
-        const float sf = mx4_scale((st.s[rt] >> sh) & 255u);
-        const uint32_t w[4] = {st.w[rt].x, st.w[rt].y, st.w[rt].z, st.w[rt].w};
+          acc[rt][mt] = mx4_mfma<0, 0>(st.w[rt], st.s[rt] >> sh, st.x[mt], st.xs[mt] >> sh, acc[rt][mt]);
+    } else {
+      // past K the rows are zero, as W is there (a load past it has read elements that may be no numbers;
+      // a select at the load would be a branch, and the loads in flight no longer counted)
+      if ((u + 1) * MX4_UNIT > a.K) {
+        const uint32_t keep = u * MX4_UNIT + r * 8 < a.K ? 0xffffffffu : 0u;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const Frag f = mx4_widen(w[j], sf);
+        for (int i = 0; i < XL; ++i)
+          st.x[i] = make_uint4(st.x[i].x & keep, st.x[i].y & keep, st.x[i].z & keep, st.x[i].w & keep);
+      }
+      // piece p of row m of a tile lies at m * 256 + (p ^ m) * 16: rows of a read and pieces of a
+      // write fall into different banks.  A wave's accesses to shared memory run in order; the empty
+      // statements keep the compiler from moving one lane's read over another lane's write.
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) acc[rt][mt] = mfma_bf16(f, st.x.f[mt][j], acc[rt][mt]);
+      for (int i = 0; i < XL; ++i) {
+        const int m = (i & 3) * 4 + g;
+        *reinterpret_cast<uint4*>(mine + (i >> 2) * 4096 + m * 256 + ((r ^ m) * 16)) = st.x[i];
+      }
+      asm volatile("" ::: "memory");
+      Frag x[4][MT];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          x[j][mt].u = *reinterpret_cast<const uint4*>(mine + mt * 4096 + r * 256 + (((g * 4 + j) ^ r) * 16));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const uint32_t w[4] = {st.w[rt].x, st.w[rt].y, st.w[rt].z, st.w[rt].w};
+          const Frag f = mx4_widen(w[j], mx4_scale((st.s[rt] >> sh) & 255u));
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) acc[rt][mt] = mfma_bf16(f, x[j][mt], acc[rt][mt]);
         }
       }
+      asm volatile("" ::: "memory");
     }
   };
 
   // this wave's run of units
-  const int per = (a.units + MR_WAVES - 1) / MR_WAVES;
+  const int per = (a.units + WAVES - 1) / WAVES;
   const int first = wave * per, last = min(a.units, first + per);
   if (first < last) {
     Stage st[STAGES];
@@ -137,7 +166,9 @@ __global__ __launch_bounds__(MR_WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a)
       if (u + d < last) compute(u + d, st[d]);
   }
 
-  // ---- the waves' sums, added in order through shared memory, one tile of outputs a round
+  // ---- the waves' sums, added in order through shared memory (a wave writes where its rows of X
+  // lay), one tile of outputs a round
+  constexpr int RED = WAVE_B / 4;
 #pragma unroll
   for (int ort = 0; ort < OUT_RT; ++ort) {
     if (ort > 0) __syncthreads();
@@ -145,20 +176,20 @@ __global__ __launch_bounds__(MR_WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a)
     for (int j = 0; j < RPR; ++j)
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt)
-        *reinterpret_cast<float4*>(red + (((wave * RPR + j) * MT + mt) * 64 + lane) * 4) =
+        *reinterpret_cast<float4*>(red + wave * RED + ((j * MT + mt) * 64 + lane) * 4) =
             make_float4(acc[ort * RPR + j][mt][0], acc[ort * RPR + j][mt][1], acc[ort * RPR + j][mt][2],
                         acc[ort * RPR + j][mt][3]);
     __syncthreads();
-    if (tid < MT * 64) {
-      const int mt = tid >> 6;
+    if (wave < MT) {
+      const int mt = wave;
       const int m = m0 + mt * 16 + r, n = (out_tile0 + ort) * 16 + 4 * g;
       float v[RPR][4];
 #pragma unroll
       for (int j = 0; j < RPR; ++j) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int w = 0; w < MR_WAVES; ++w) {
-          const float4 p = *reinterpret_cast<const float4*>(red + (((w * RPR + j) * MT + mt) * 64 + lane) * 4);
+        for (int w = 0; w < WAVES; ++w) {
+          const float4 p = *reinterpret_cast<const float4*>(red + w * RED + ((j * MT + mt) * 64 + lane) * 4);
           s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
         }
         v[j][0] = s.x; v[j][1] = s.y; v[j][2] = s.z; v[j][3] = s.w;
@@ -182,21 +213,42 @@ __global__ __launch_bounds__(MR_WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a)
   }
 }
 
-template <int MT, int RT, int STAGES, int EPI, typename OutT, bool X4>
+template <int WAVES, int MT, int XQ, int RT, int STAGES, int EPI, typename OutT, bool X4>
 static int launch_mx4_rows(const Mx4Args& a) {
   constexpr int OUT_RT = EPI == MR_EPI_GATED ? RT / 2 : RT;
   const int tiles = (a.n_out + 15) / 16;
   const dim3 grid((tiles + OUT_RT - 1) / OUT_RT, (a.M + 16 * MT - 1) / (16 * MT));
   if (grid.y > 65535) return LLM_ERR_ARG;
-  gemm_mx4_rows_kernel<MT, RT, STAGES, EPI, OutT, X4><<<grid, MR_WAVES * 64, 0, a.stream>>>(a);
+  gemm_mx4_rows_kernel<WAVES, MT, XQ, RT, STAGES, EPI, OutT, X4><<<grid, WAVES * 64, 0, a.stream>>>(a);
   return llm_launch_status();
+}
+
+// How many waves split K depends on W alone (an output's sum does not change with the batch): 16
+// where there are tiles of outputs for half of the compute units at most, 8 up to one a unit, else 4,
+// whose longer runs overlap better (us, 4 / 8 / 16 waves: 2,048 x 2,048 by 16 rows 4.6 / 4.6 / 3.9;
+// 14,336 x 4,096 by one row 9.7 / 8.6 / 8.8; 4,096 x 6,144 by 16 rows 9.6 / 11.6 / 11.2; gate and up
+// of 4,096 x 14,336 by 8 rows 20.2 / 26.1 / 28.5).  Two tiles of outputs a wave halve what a block
+// reads of X: from 9 rows on, where tiles are many (that gate and up: 23.0 against 24.1 us by 16 rows,
+// but 17.9 against 16.3 by one).
+template <int MT, int XQ, int STAGES, int EPI, typename OutT, bool X4>
+static int pick_mx4_tiles(const Mx4Args& a) {
+  constexpr int ONE = EPI == MR_EPI_GATED ? 2 : 1;
+  const int tiles = (a.n_out + 15) / 16, units = llm_compute_units();
+  if (tiles <= units / 2) return launch_mx4_rows<16, MT, XQ, ONE, 2, EPI, OutT, X4>(a);
+  if (tiles <= units) return launch_mx4_rows<8, MT, XQ, ONE, STAGES, EPI, OutT, X4>(a);
+  if constexpr (MT == 1 && XQ == 4 && !X4)
+    if (tiles >= 3 * units) return launch_mx4_rows<4, MT, XQ, 2 * ONE, STAGES, EPI, OutT, X4>(a);
+  return launch_mx4_rows<4, MT, XQ, ONE, STAGES, EPI, OutT, X4>(a);
 }
 
 template <int EPI, typename OutT, bool X4>
 static int pick_mx4_rows(const Mx4Args& a) {
-  if (a.M <= 16) return launch_mx4_rows<1, 2, 4, EPI, OutT, X4>(a);
-  if (a.M <= 32) return launch_mx4_rows<2, 2, 2, EPI, OutT, X4>(a);
-  return launch_mx4_rows<4, 2, 2, EPI, OutT, X4>(a);
+  if constexpr (!X4) {
+    if (a.M <= 4) return pick_mx4_tiles<1, 1, 4, EPI, OutT, X4>(a);
+    if (a.M <= 8) return pick_mx4_tiles<1, 2, 4, EPI, OutT, X4>(a);
+  }
+  if (a.M <= 16) return pick_mx4_tiles<1, 4, 4, EPI, OutT, X4>(a);
+  return pick_mx4_tiles<2, 4, 3, EPI, OutT, X4>(a);
 }
 
 template <bool X4>

@@ -10,9 +10,9 @@
 // v_mfma_scale_f32_16x16x128_f8f6f4, and word j of every piece is the operand of one
 // v_mfma_f32_16x16x32_bf16 once it is widened (its slots of K then stand for the elements
 // 32 (l / 16) + 8 j .. + 7 of the unit, for which the other operand is read the same way).  A wave's
-// load of a unit is 1 KiB in a row.  The scales of four units in a row lie together, a word a lane:
-// byte u % 4 of word ((tile * quads + u / 4) * 64 + lane).  Rows, blocks and elements that pad a
-// tile are zero.
+// load of a unit is 1 KiB in a row.  The scales of four units in a row (a quad) lie together, a word
+// a lane: byte u % 4 of word ((tile * quads + u / 4) * 64 + lane).  A tile has whole quads; rows,
+// blocks and elements that pad it are zero.
 #pragma once
 #include "mfma.h"
 

@@ -30,7 +30,7 @@ __device__ __forceinline__ void block_load(const T* p, int n, float (&v)[MX4_BLO
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__ X, size_t ldx, int M, int K,
                                                            uint4* __restrict__ codes, uint32_t* __restrict__ scales,
-                                                           int units, int quads) {
+                                                           int quads) {
   const int lane = threadIdx.x & 63, quad = blockIdx.y * 4 + (threadIdx.x >> 6);
   const int tile = blockIdx.x, r = lane & 15, g = lane >> 4;
   if (quad >= quads) return;
@@ -39,7 +39,6 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int u = quad * 4 + i;
-    if (u >= units) break;
     const int k = u * MX4_UNIT + g * MX4_BLOCK;
     const int n = row < M ? K - k : 0;
     float v[MX4_BLOCK];
@@ -60,7 +59,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__
       c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[8 * j + 6], v[8 * j + 7], sf, 3);
       w[j] = c;
     }
-    codes[((size_t)tile * units + u) * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+    codes[((size_t)tile * quads * 4 + u) * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
     sw |= scale << (8 * i);
   }
   scales[((size_t)tile * quads + quad) * 64 + lane] = sw;
@@ -69,7 +68,7 @@ __global__ __launch_bounds__(256) void mx4_quantize_kernel(const T* __restrict__
 template <typename T, bool WIDE>
 __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint4* __restrict__ codes,
                                                              const uint32_t* __restrict__ scales, T* __restrict__ out,
-                                                             int M, int K, int units, int quads) {
+                                                             int M, int K, int quads) {
   const int lane = threadIdx.x & 63, quad = blockIdx.y * 4 + (threadIdx.x >> 6);
   const int tile = blockIdx.x, r = lane & 15, g = lane >> 4;
   const int row = tile * 16 + r;
@@ -79,8 +78,8 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint4* __rest
   for (int i = 0; i < 4; ++i) {
     const int u = quad * 4 + i;
     const int k = u * MX4_UNIT + g * MX4_BLOCK, n = K - k;
-    if (u >= units || n <= 0) break;
-    const uint4 c = codes[((size_t)tile * units + u) * 64 + lane];
+    if (n <= 0) break;
+    const uint4 c = codes[((size_t)tile * quads * 4 + u) * 64 + lane];
     const uint32_t w[4] = {c.x, c.y, c.z, c.w};
     const float sf = mx4_scale((sw >> (8 * i)) & 255u);
     float v[MX4_BLOCK];
@@ -112,7 +111,7 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint4* __rest
 __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* __restrict__ rows, size_t ldc,
                                                        const uint8_t* __restrict__ row_scales, int N, int K,
                                                        uint4* __restrict__ codes, uint32_t* __restrict__ scales,
-                                                       int units, int quads) {
+                                                       int quads) {
   const int lane = threadIdx.x & 63, quad = blockIdx.y * 4 + (threadIdx.x >> 6);
   const int tile = blockIdx.x, r = lane & 15, g = lane >> 4;
   if (quad >= quads) return;
@@ -120,7 +119,6 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* __restrict
   uint32_t sw = 0;
   for (int i = 0; i < 4; ++i) {
     const int u = quad * 4 + i, b = u * 4 + g;
-    if (u >= units) break;
     uint32_t w[4] = {0, 0, 0, 0};
     if (row < N && b < blocks) {
       const uint8_t* src = rows + (size_t)row * ldc + b * 16;
@@ -133,7 +131,7 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* __restrict
       }
       sw |= (uint32_t)row_scales[(size_t)row * blocks + b] << (8 * i);
     }
-    codes[((size_t)tile * units + u) * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
+    codes[((size_t)tile * quads * 4 + u) * 64 + lane] = make_uint4(w[0], w[1], w[2], w[3]);
   }
   scales[((size_t)tile * quads + quad) * 64 + lane] = sw;
 }
@@ -149,7 +147,7 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(const bf16_t* __restrict_
 
 static inline dim3 mx4_grid(int rows, int k) { return dim3(mx4_tiles(rows), (mx4_quads(k) + 3) / 4); }
 
-// X [M, K] of `dtype`, rows ldx elements apart, into codes (mx4_tiles(M) * mx4_units(K) * 1024 bytes)
+// X [M, K] of `dtype`, rows ldx elements apart, into codes (mx4_tiles(M) * mx4_quads(K) * 4096 bytes)
 // and scales (mx4_tiles(M) * mx4_quads(K) * 256 bytes).
 extern "C" int llm_mx4_quantize(const void* X, int dtype, size_t ldx, int M, int K, void* codes, void* scales,
                                 hipStream_t stream) {
@@ -157,10 +155,10 @@ extern "C" int llm_mx4_quantize(const void* X, int dtype, size_t ldx, int M, int
   if ((((uintptr_t)codes) | ((uintptr_t)scales)) & 15) return LLM_ERR_ARG;
   const dim3 grid = mx4_grid(M, K);
   if (grid.y > 65535) return LLM_ERR_ARG;
-  const int units = mx4_units(K), quads = mx4_quads(K);
+  const int quads = mx4_quads(K);
   const bool wide = (ldx & 3) == 0 && (((uintptr_t)X) & (dtype == LLM_DTYPE_F32 ? 15 : 7)) == 0;
 #define MX4_LAUNCH(T, W) \
-  mx4_quantize_kernel<T, W><<<grid, 256, 0, stream>>>((const T*)X, ldx, M, K, (uint4*)codes, (uint32_t*)scales, units, quads)
+  mx4_quantize_kernel<T, W><<<grid, 256, 0, stream>>>((const T*)X, ldx, M, K, (uint4*)codes, (uint32_t*)scales, quads)
   if (dtype == LLM_DTYPE_F32) {
     if (wide) MX4_LAUNCH(float, true); else MX4_LAUNCH(float, false);
   } else if (dtype == LLM_DTYPE_BF16) {
@@ -178,10 +176,10 @@ extern "C" int llm_mx4_dequantize(const void* codes, const void* scales, void* o
   if ((((uintptr_t)codes) | ((uintptr_t)scales)) & 15) return LLM_ERR_ARG;
   const dim3 grid = mx4_grid(M, K);
   if (grid.y > 65535) return LLM_ERR_ARG;
-  const int units = mx4_units(K), quads = mx4_quads(K);
+  const int quads = mx4_quads(K);
   const bool wide = (K & 3) == 0 && (((uintptr_t)out) & 15) == 0;
 #define MX4_LAUNCH(T, W) \
-  mx4_dequantize_kernel<T, W><<<grid, 256, 0, stream>>>((const uint4*)codes, (const uint32_t*)scales, (T*)out, M, K, units, quads)
+  mx4_dequantize_kernel<T, W><<<grid, 256, 0, stream>>>((const uint4*)codes, (const uint32_t*)scales, (T*)out, M, K, quads)
   if (dtype == LLM_DTYPE_F32) {
     if (wide) MX4_LAUNCH(float, true); else MX4_LAUNCH(float, false);
   } else if (dtype == LLM_DTYPE_BF16) {
@@ -202,7 +200,7 @@ extern "C" int llm_mx4_pack(const void* rows, size_t ldc, const void* row_scales
   const dim3 grid = mx4_grid(N, K);
   if (grid.y > 65535) return LLM_ERR_ARG;
   mx4_pack_kernel<<<grid, 256, 0, stream>>>((const uint8_t*)rows, ldc, (const uint8_t*)row_scales, N, K, (uint4*)codes,
-                                            (uint32_t*)scales, mx4_units(K), mx4_quads(K));
+                                            (uint32_t*)scales, mx4_quads(K));
   return llm_launch_status();
 }
 

@@ -14,7 +14,7 @@ from ..errors import KernelError
 _vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 
 BLOCK = 32              # elements that share a scale
-TILE_ROWS, UNIT = 16, 128
+TILE_ROWS, QUAD = 16, 512      # a tile holds 16 rows by whole quads of 512 elements
 
 SIGNATURES = {
     "llm_mx4_quantize": [_vp, _i, _sz, _i, _i, _vp, _vp, _vp],
@@ -22,13 +22,14 @@ SIGNATURES = {
     "llm_mx4_pack": [_vp, _sz, _vp, _i, _i, _vp, _vp, _vp],
     "llm_pad_rows": [_vp, _sz, _vp, _i, _i, _i, _vp],
     "llm_gemm_mx4_rows": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "llm_gemm_mx4_many": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
 }
 
 
 def tiled_sizes(rows: int, width: int):
     """(bytes of codes, bytes of scales) of a matrix of these sizes, whole tiles."""
-    tiles, units = -(-rows // TILE_ROWS), -(-width // UNIT)
-    return tiles * units * 1024, tiles * -(-units // 4) * 256
+    tiles, quads = -(-rows // TILE_ROWS), -(-width // QUAD)
+    return tiles * quads * 4096, tiles * quads * 256
 
 
 class Mx4Matrix:
@@ -55,6 +56,8 @@ class Mx4Matrix:
 
 class Mx4Ops:
     """The operations of ``HipOps`` on matrices in MXFP4."""
+
+    MX4_ROWS = 32           # most rows that go to the product for few rows
 
     def _mx4_empty(self, rows, width):
         if rows <= 0 or width <= 0:
@@ -113,10 +116,10 @@ class Mx4Ops:
                                           q.codes.data_ptr(), q.scales.data_ptr(), self._stream()), "mx4_from_codes")
         return q
 
-    def _mx4_rows(self, x, k):
-        """Rows for a product with an MXFP4 weight: (pointer, pointer to scales or None, row
-        stride, what keeps them alive).  bfloat16 rows whose length or address does not allow
-        loads of 16 bytes are copied to a padded buffer first."""
+    def _mx4_rows(self, x, k, piece):
+        """Rows for a product with an MXFP4 weight that reads ``piece`` elements of them at a time:
+        (pointer, pointer to scales or None, row stride, what keeps them alive).  bfloat16 rows
+        whose length, distance or address does not allow that are copied to a padded buffer first."""
         if isinstance(x, Mx4Matrix):
             codes, scales = self._mx4(x, "linear input")
             return codes, scales, 0, x
@@ -127,9 +130,9 @@ class Mx4Ops:
         if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < k):
             raise KernelError("linear input must be a matrix with contiguous rows")
         ld = max(x.stride(0), k)
-        if k % 8 == 0 and ld % 8 == 0 and x.data_ptr() % 16 == 0:
+        if k % piece == 0 and ld % piece == 0 and x.data_ptr() % 16 == 0:
             return x.data_ptr(), None, ld, x
-        ldp = -(-k // 8) * 8
+        ldp = -(-k // piece) * piece
         padded = torch.empty((x.shape[0], ldp), dtype=torch.bfloat16, device=self.device)
         self._check(self.lib.llm_pad_rows(x.data_ptr(), ld, padded.data_ptr(), x.shape[0], k, ldp, self._stream()),
                     "pad_rows")
@@ -142,11 +145,14 @@ class Mx4Ops:
         codes, scales = self._mx4(w, "MXFP4 weight")
         if m == 0:
             return out
-        xp, xs, ldx, alive = self._mx4_rows(x, k)
+        many = m > self.MX4_ROWS
+        piece = 128 if many else 8
+        xp, xs, ldx, alive = self._mx4_rows(x, k, piece)
         bptr = None if bias is None else self._dev(bias, "bias", torch.float32, (n,))
-        # (the rows are padded to 8 elements where K is not a multiple of it: the weight's codes there are zero)
-        self._check(self.lib.llm_gemm_mx4_rows(xp, xs, ldx, codes, scales, bptr, out.data_ptr(), epilogue, _code(out.dtype),
-                                               m, n, -(-k // 8) * 8, self._stream()), "gemm_mx4_rows")
+        # (where rows were padded, K is their padded length: the weight's codes there are zero)
+        fn = self.lib.llm_gemm_mx4_many if many else self.lib.llm_gemm_mx4_rows
+        self._check(fn(xp, xs, ldx, codes, scales, bptr, out.data_ptr(), epilogue, _code(out.dtype), m, n,
+                       -(-k // piece) * piece, self._stream()), "gemm_mx4_many" if many else "gemm_mx4_rows")
         return out
 
     def _linear_mx4(self, x, w, bias, out_dtype, residual=None):
