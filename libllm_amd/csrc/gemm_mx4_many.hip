@@ -24,6 +24,9 @@
 
 #include <type_traits>
 
+// The kernel is written in lambdas over fixed arrays of registers: each has to go into the kernel whole.
+#define MM_INLINE __attribute__((always_inline))
+
 #define MM_EPI_NONE 0
 #define MM_EPI_GATED 1
 
@@ -38,6 +41,7 @@ struct Mx4ManyArgs {
   int M, N, n_out;
   int ldx, units, quads, act;
   int m_tiles, n_tiles;      // blocks along X and W
+  int slice_quads;           // quads of K a slice (blockIdx.y counts them); one slice has them all
   hipStream_t stream;
 };
 
@@ -59,19 +63,23 @@ __device__ __forceinline__ void lds_fill(uint32_t lds, const void* base, uint32_
                : "=&s"(m0_was) : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 
-template <bool X4, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
+template <bool X4, int NBUF, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
   constexpr int NW = WM * WN;
   constexpr int BM = WM * MTW * 16, BNT = WN * NTW;         // rows of X, tiles of W a block
   constexpr int STEPS = X4 ? 2 : 4;
   constexpr int XB = X4 ? BM * 128 : BM * 256;              // bytes of X's tile of K
-  constexpr int WB = X4 ? BNT * 2048 : 0;                   // of W's, where it goes through LDS
+  constexpr bool WL = X4 || NBUF > 2;                       // W's codes and scales go through LDS
+  constexpr int WB = X4 ? BNT * 2048 : WL ? BNT * 1024 : 0;
   constexpr int BUF = XB + WB;
-  constexpr int TILES = BM / 16 + BNT;
-  constexpr int SB = X4 ? TILES * 256 : 0;                  // scales of a quad: W's tiles, then X's
-  constexpr int FILLS = BUF / 1024 / NW;                    // 1 KiB each
-  static_assert(BUF % (1024 * NW) == 0, "every wave fills as much");
+  constexpr int STILES = X4 ? BM / 16 + BNT : WL ? BNT : 0; // tiles whose scales do: W's, then X's
+  constexpr int SB = STILES * 256;                          // scales of a quad
+  constexpr int TPQ = X4 ? 2 : 4;                           // tiles of K a quad
+  constexpr int NSB = NBUF > TPQ + 1 ? 4 : 2;               // quads of scales held
+  constexpr int TURNS = WL && TPQ > NBUF ? TPQ : NBUF;      // rounds after which all of these repeat
+  constexpr int XF = XB / 1024 / NW, FILLS = BUF / 1024 / NW;       // loads of 1 KiB a wave and tile: X's, all
+  static_assert(XB % (1024 * NW) == 0 && BUF % (1024 * NW) == 0 && TURNS % 2 == 0, "every wave fills as much");
   constexpr bool GATED = EPI == MM_EPI_GATED;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
@@ -89,65 +97,81 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   const int out_tiles = (a.n_out + 15) / 16;
 
   // tile of W that is number t of this block (past the end the last one; its sums are not stored)
-  auto w_tile = [&](int t) {
+  auto w_tile = [&](int t) MM_INLINE {
     if (GATED) return min(nt_blk * (BNT / 2) + t % (BNT / 2), out_tiles - 1) + (t / (BNT / 2)) * out_tiles;
     return min(nt_blk * BNT + t, out_tiles - 1);
   };
   // number within the block of tile nt of this wave: gated, its gate tiles and then its up tiles
-  auto wave_tile = [&](int nt) {
+  auto wave_tile = [&](int nt) MM_INLINE {
     return GATED ? (nt / (NTW / 2)) * (BNT / 2) + wn * (NTW / 2) + nt % (NTW / 2) : wn * NTW + nt;
   };
   const size_t c_tile = (size_t)a.quads * 4096, s_tile = (size_t)a.quads * 256;
+  // K may be a slice, a run of whole quads: everything begins that far into its rows, and the sums go
+  // to a matrix of the slice's own (plain epilogue in float32), to be added in order by whoever reads them
+  const int q0 = blockIdx.y * a.slice_quads;
+  const int units = min(a.units - 4 * q0, 4 * a.slice_quads), quads = min(a.quads - q0, a.slice_quads);
+  a.X += (size_t)q0 * 512;
+  a.xc += (size_t)q0 * 4096;
+  a.wc += (size_t)q0 * 4096;
+  a.xs += (size_t)q0 * 256;
+  a.ws += (size_t)q0 * 256;
+  a.C = (OutT*)a.C + (size_t)blockIdx.y * a.M * a.n_out;
 
   // ---- what this wave fills, and where from
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)lds;
   static_assert(X4 || NW % 4 == 0, "the rows a wave fills lie a multiple of 16 apart");
   const uint32_t lane16 = lane * 16, lane4 = lane * 4;
-  const uint8_t* fill_base[X4 ? FILLS : 1];
+  const uint8_t* fill_base[FILLS];
   int fill_row = 0;
   uint32_t fill_piece = 0;
-  if constexpr (X4) {
 #pragma unroll
-    for (int p = 0; p < FILLS; ++p) {
-      const int c = p * NW + wave, t = c >> 1;              // which KiB of the buffer: (tile, unit) of X, then of W
-      fill_base[p] = (t < BM / 16 ? a.xc + (size_t)min(m0 / 16 + t, (a.M - 1) / 16) * c_tile
-                                  : a.wc + (size_t)w_tile(t - BM / 16) * c_tile) + (c & 1) * 1024;
+  for (int p = 0; p < FILLS; ++p) {
+    const int c = p * NW + wave;                            // which KiB of the buffer
+    if (X4) {                                               // (tile, unit) of X, then of W
+      const int t = c >> 1;
+      fill_base[p] = (p < XF ? a.xc + (size_t)min(m0 / 16 + t, (a.M - 1) / 16) * c_tile
+                             : a.wc + (size_t)w_tile(t - BM / 16) * c_tile) + (c & 1) * 1024;
+    } else {                                                // four rows of X; a tile of W
+      fill_base[p] = p < XF ? (const uint8_t*)(a.X + (size_t)m0 * a.ldx) : a.wc + (size_t)w_tile(c - XB / 1024) * c_tile;
     }
-  } else {                                                  // four rows of X
-    fill_base[0] = (const uint8_t*)(a.X + (size_t)m0 * a.ldx);
+  }
+  if constexpr (!X4) {
     fill_row = wave * 4 + g;
     fill_piece = (r ^ (fill_row & 15)) * 16;
   }
   // scales of a quad: a KiB is four tiles; waves beyond them fill what another wave fills, with the same
-  constexpr int SC_WAVES = TILES / 4;
-  static_assert(!X4 || (TILES % 4 == 0 && SC_WAVES <= NW), "a wave fills the scales of four tiles at most");
-  const int sc_wave = X4 ? wave % SC_WAVES : 0;
+  constexpr int SC_WAVES = WL ? STILES / 4 : 1;
+  static_assert(STILES % 4 == 0 && SC_WAVES <= NW, "a wave fills the scales of four tiles at most");
+  const int sc_wave = __builtin_amdgcn_readfirstlane(wave % SC_WAVES);
   const uint8_t* sc_base = nullptr;
-  if constexpr (X4) {
+  if constexpr (WL) {
     const int t = sc_wave * 4 + (lane >> 4);
     sc_base = (t < BNT ? a.ws + (size_t)w_tile(t) * s_tile
                        : a.xs + (size_t)min(m0 / 16 + t - BNT, (a.M - 1) / 16) * s_tile) + (lane & 15) * 16;
   }
-  const int n_kt = X4 ? (a.units + 1) / 2 : a.units;
+  const int n_kt = X4 ? (units + 1) / 2 : units;
   // Tile kt of K into buffer `buf`; past the last tile the last one again, which nobody reads: the
   // loop has no branch then, over which the compiler would move matrix instructions.
-  auto fill = [&](int kt, int buf, int p) {
+  auto fill = [&](int kt, int buf, int p) MM_INLINE {
     const uint32_t at = lds0 + buf * BUF + (p * NW + wave) * 1024;
-    if constexpr (X4) {
-      lds_fill(at, fill_base[p] + (size_t)min(kt, n_kt - 1) * 2048, lane16);
+    const size_t k = min(kt, n_kt - 1);
+    if (X4) {
+      lds_fill(at, fill_base[p] + k * 2048, lane16);
+    } else if (p >= XF) {
+      lds_fill(at, fill_base[p] + k * 1024, lane16);
     } else {                                                // (the offset made anew each time: held, it would cost a register a fill)
       int row = fill_row;
       asm volatile("" : "+v"(row));
       row = min(row + p * NW * 4, a.M - 1 - m0);
-      lds_fill(at, fill_base[0] + (size_t)min(kt, n_kt - 1) * 256, (uint32_t)row * (uint32_t)a.ldx * 2 + fill_piece);
+      lds_fill(at, fill_base[p] + k * 256, (uint32_t)row * (uint32_t)a.ldx * 2 + fill_piece);
     }
   };
-  auto fill_scales = [&](int q, int buf) {
-    if constexpr (X4) {
+  auto fill_scales = [&](int q) MM_INLINE {
+    if constexpr (WL) {
       uint32_t m0_was;
       asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
-                   : "=&s"(m0_was) : "s"(lds0 + 2 * BUF + buf * SB + sc_wave * 1024),
-                     "v"(sc_base + (size_t)min(q, a.quads - 1) * 256) : "memory");
+                   : "=&s"(m0_was) : "s"(lds0 + NBUF * BUF + (q & (NSB - 1)) * SB + sc_wave * 1024),
+                     "v"(sc_base + (size_t)min(q, quads - 1) * 256) : "memory");
     }
   };
 
@@ -170,33 +194,36 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   const uint32_t w_lane = lds0 + XB + lane16;
   typedef const __attribute__((address_space(3))) u4_raw* lds_u4;
   typedef const __attribute__((address_space(3))) uint16_t* lds_u2;
+  typedef const __attribute__((address_space(3))) uint8_t* lds_u1;
   typedef const __attribute__((address_space(1))) u4_raw* global_u4;
   typedef const __attribute__((address_space(1))) uint32_t* global_u1;
-  auto plus = [&](uint32_t lane_at, int by) {
+  auto plus = [&](uint32_t lane_at, int by) MM_INLINE {
     uint32_t at;
     asm volatile("v_add_u32 %0, %1, %2" : "=v"(at) : "s"(by), "v"(lane_at));
     return at;
   };
-  auto x_step = [&](int buf, int step) {                    // (piece 4 g + step of row r lies at its xor with r)
+  auto x_step = [&](int buf, int step) MM_INLINE {                    // (piece 4 g + step of row r lies at its xor with r)
     uint32_t at = x_lane;
     if constexpr (!X4) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(at) : "s"(step * 16), "v"(x_lane));
     return plus(at, buf * BUF + (X4 ? step * 1024 : 0));
   };
-  auto lds_read = [&](uint32_t at) {
+  auto lds_read = [&](uint32_t at) MM_INLINE {
     const u4_raw v = *(lds_u4)(uintptr_t)at;
     Frag f;
     f.u = make_uint4(v.x, v.y, v.z, v.w);
     return f;
   };
-  auto read_x = [&](uint32_t at, int mt) { return lds_read(at + mt * (X4 ? 2048 : 4096)); };
-  auto read_w = [&](uint32_t at, int nt) { return lds_read(at + wave_tile(nt) * 2048); };
-  auto read_scales = [&](uint32_t at, int i, uint32_t& lo, uint32_t& hi) {      // word i: tiles 2 i and 2 i + 1, W's first
+  auto read_x = [&](uint32_t at, int mt) MM_INLINE { return lds_read(at + mt * (X4 ? 2048 : 4096)); };
+  auto read_w = [&](uint32_t at, int nt) MM_INLINE { return lds_read(at + wave_tile(nt) * 2048); };
+  auto read_scales = [&](uint32_t at, int i, uint32_t& lo, uint32_t& hi) MM_INLINE {      // word i: tiles 2 i and 2 i + 1, W's first
     const int t0 = 2 * i < NTW ? wave_tile(2 * i) : BNT + wm * MTW + 2 * i - NTW;
     const int t1 = 2 * i < NTW ? wave_tile(2 * i + 1) : t0 + 1;
     lo = *(lds_u2)(uintptr_t)(at + t0 * 256);
     hi = *(lds_u2)(uintptr_t)(at + t1 * 256);
   };
-  auto load_w = [&](int kt, int set) {
+  auto read_codes = [&](uint32_t at, int nt) MM_INLINE { return *(lds_u4)(uintptr_t)(at + wave_tile(nt) * 1024); };
+  auto read_scale = [&](uint32_t at, int nt) MM_INLINE { return (uint32_t) * (lds_u1)(uintptr_t)(at + wave_tile(nt) * 256); };
+  auto load_w = [&](int kt, int set) MM_INLINE {
 #pragma unroll
     for (int nt = 0; nt < NTW; ++nt) {
       const size_t t = w_tile(wave_tile(nt));
@@ -208,20 +235,24 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     }
   };
 
-  each<FILLS>([&](auto p) { fill(0, 0, p); });
-  fill_scales(0, 0);
-  each<FILLS>([&](auto p) { fill(1, 1, p); });
+  each<NBUF>([&](auto b) MM_INLINE {
+    if (b % TPQ == 0) fill_scales(b / TPQ);
+    each<FILLS>([&](auto p) MM_INLINE { fill(b, b, p); });
+  });
   // (the compiler is told that it has W's codes: else it would wait for them, and with them for every
   // load into LDS behind them, inside the loop)
-  auto have_w = [&](int set) {
+  auto have_w = [&](int set) MM_INLINE {
 #pragma unroll
     for (int nt = 0; nt < NTW; ++nt) asm volatile("" : "+v"(wc[set][nt]), "+v"(wsc[set][nt]));
   };
-  if constexpr (!X4) {
+  if constexpr (!WL) {
     load_w(0, 0);
     have_w(0);
   }
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // everything this wave asked for has arrived
+  // What this wave asked for has arrived, but for the loads of that many tiles, the last ones.
+#define MM_ARRIVED(TILES) \
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(WL ? (TILES)*FILLS : 0) : "memory")
+  MM_ARRIVED(NBUF - 1);
   __syncthreads();
   {
     const uint32_t x_at = x_step(0, 0);
@@ -234,49 +265,55 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
 #pragma unroll
     for (int i = 0; i < (NTW + MTW) / 2; ++i) {
       uint32_t lo, hi;
-      read_scales(lds0 + 2 * BUF + lane4, i, lo, hi);
+      read_scales(lds0 + NBUF * BUF + lane4, i, lo, hi);
       sc[0][i] = lo | hi << 16;
+    }
+  } else if constexpr (WL) {
+#pragma unroll
+    for (int nt = 0; nt < NTW; ++nt) {
+      wc[0][nt] = read_codes(w_lane, nt);
+      wsc[0][nt] = read_scale(lds0 + NBUF * BUF + lane4, nt);
     }
   }
 
-  // one tile of K; CUR: which set of scales (or codes of W) is its own, and the buffer it lies in
-  auto round = [&](int kt, auto cur) {
-    constexpr int CUR = decltype(cur)::value, NEXT = CUR ^ 1;
+  // One tile of K, the turn-th of TURNS; CUR: which set of scales (or codes of W) is its own.
+  auto round = [&](int kt, auto turn) MM_INLINE {
+    constexpr int TURN = decltype(turn)::value, CUR = TURN & 1, NEXT = CUR ^ 1;
     uint32_t sc_lo[(NTW + MTW) / 2], sc_hi[(NTW + MTW) / 2];
-    if constexpr (!X4) load_w(min(kt + 1, n_kt - 1), NEXT);
-    each<STEPS>([&](auto step) {
+    if constexpr (!WL) load_w(min(kt + 1, n_kt - 1), NEXT);
+    each<STEPS>([&](auto step) MM_INLINE {
       constexpr int S = decltype(step)::value, SET = S & 1;
       constexpr bool LAST = S == STEPS - 1;
-      constexpr int RBUF = LAST ? NEXT : CUR, RS = LAST ? 0 : S + 1;      // where the next step's fragments lie
+      constexpr int RBUF = (TURN + LAST) % NBUF, RS = LAST ? 0 : S + 1;      // where the next step's fragments lie
       if constexpr (LAST) {
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (!X4) have_w(NEXT);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if constexpr (!WL) have_w(NEXT);
+        MM_ARRIVED(NBUF - 2);
         __syncthreads();
       }
       const uint32_t x_at = x_step(RBUF, RS);
       uint32_t w_at = 0, s_at = 0;
       Frag w[X4 ? 1 : NTW];
-      if constexpr (X4) {
-        w_at = plus(w_lane, RBUF * BUF + RS * 1024);
-        if constexpr (LAST) s_at = plus(lane4, lds0 + 2 * BUF + (((kt + 1) >> 1) & 1) * SB + NEXT * 2);
-      } else {
-        const int sh = 8 * (kt & 3);
-#pragma unroll
-        for (int nt = 0; nt < NTW; ++nt) {
-          w[nt] = mx4_widen(wc[CUR][nt][S], mx4_scale((wsc[CUR][nt] >> sh) & 255u));
-        }
+      if constexpr (WL) {
+        if constexpr (X4 || LAST) w_at = plus(w_lane, RBUF * BUF + (X4 ? RS * 1024 : 0));
+        if constexpr (LAST)
+          s_at = plus(lane4, lds0 + NBUF * BUF + (((kt + 1) / TPQ) & (NSB - 1)) * SB + (TURN + 1) % TPQ * (X4 ? 2 : 1));
       }
-      each<MTW>([&](auto mtc) {
+      if constexpr (!X4) {
+        const int sh = WL ? 0 : 8 * (kt & 3);
+#pragma unroll
+        for (int nt = 0; nt < NTW; ++nt) w[nt] = mx4_widen(wc[CUR][nt][S], mx4_scale((wsc[CUR][nt] >> sh) & 255u));
+      }
+      each<MTW>([&](auto mtc) MM_INLINE {
         constexpr int MT = decltype(mtc)::value;
         __builtin_amdgcn_sched_barrier(0);
-        // this group's share of the loads of the tile after next
+        // this group's share of the loads into the buffer that is left
         if constexpr (LAST) {
+          if (MT == 0 && (TURN + NBUF) % TPQ == 0) fill_scales((kt + NBUF) / TPQ);
 #pragma unroll
-          for (int p = FILLS * MT / MTW; p < FILLS * (MT + 1) / MTW; ++p) fill(kt + 2, CUR, p);
-          if (MT == 0 && CUR == 0) fill_scales((kt + 2) >> 1, ((kt + 2) >> 1) & 1);
+          for (int p = FILLS * MT / MTW; p < FILLS * (MT + 1) / MTW; ++p) fill(kt + NBUF, TURN % NBUF, p);
         }
-        each<NTW>([&](auto ntc) {
+        each<NTW>([&](auto ntc) MM_INLINE {
           constexpr int NT = decltype(ntc)::value;
           if constexpr (X4)
             acc[NT][MT] = mx4_mfma<(NT & 1) * 2 + S, (MT & 1) * 2 + S>(wf[SET][NT].u, sc[CUR][NT / 2], xf[MT].u,
@@ -295,6 +332,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
 #pragma unroll
             for (int i = NS * MT / MTW; i < NS * (MT + 1) / MTW; ++i) read_scales(s_at, i, sc_lo[i], sc_hi[i]);
           }
+        } else if constexpr (WL && LAST) {
+#pragma unroll
+          for (int nt = NTW * MT / MTW; nt < NTW * (MT + 1) / MTW; ++nt) {
+            wc[NEXT][nt] = read_codes(w_at, nt);
+            wsc[NEXT][nt] = read_scale(s_at, nt);
+          }
         }
       });
     });
@@ -306,11 +349,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   };
   static_assert(STEPS % 2 == 0, "a tile of K ends on the set of W's fragments that it began with");
   int kt = 0;
-  for (; kt + 2 <= n_kt; kt += 2) {
-    round(kt, std::integral_constant<int, 0>{});
-    round(kt + 1, std::integral_constant<int, 1>{});
-  }
-  if (kt < n_kt) round(kt, std::integral_constant<int, 0>{});
+  for (; kt + TURNS <= n_kt; kt += TURNS) each<TURNS>([&](auto turn) MM_INLINE { round(kt + turn, turn); });
+  each<TURNS - 1>([&](auto turn) MM_INLINE {
+    if (kt + turn < n_kt) round(kt + turn, turn);
+  });
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // the last loads into LDS have landed too
 
   // ---- epilogue: lane holds C[m = .. + r][n = .. + 4 g + e]
@@ -324,7 +366,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
       const int n = n_wave + nt * 16 + 4 * g + e;
       bias[nt][e] = !GATED && a.bias != nullptr && n < a.n_out ? a.bias[n] : 0.f;
     }
-  auto value = [&](int nt, int mt, float (&v)[4]) {
+  auto value = [&](int nt, int mt, float (&v)[4]) MM_INLINE {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[e] = acc[nt][mt][e];
@@ -399,13 +441,15 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   }
 }
 
-template <bool X4, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
+template <bool X4, int NBUF, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
 static int launch_mx4_many(Mx4ManyArgs a) {
   constexpr int BM = WM * MTW * 16, BNT = WN * NTW, NW = WM * WN;
-  constexpr int BUF = X4 ? BM * 128 + BNT * 2048 : BM * 256, SB = X4 ? (BM / 16 + BNT) * 256 : 0;
+  constexpr bool WL = X4 || NBUF > 2;                        // (sizes as in the kernel)
+  constexpr int BUF = X4 ? BM * 128 + BNT * 2048 : BM * 256 + (WL ? BNT * 1024 : 0);
+  constexpr int SB = (X4 ? BM / 16 + BNT : WL ? BNT : 0) * 256, NSB = NBUF > (X4 ? 2 : 4) + 1 ? 4 : 2;
   constexpr int OUT_NT = EPI == MM_EPI_GATED ? NTW / 2 : NTW;
   constexpr int TURN = NW * 16 * (OUT_NT * 32 + 16);
-  constexpr int LDS_BYTES = 2 * (BUF + SB) > TURN ? 2 * (BUF + SB) : TURN;
+  constexpr int HELD = NBUF * BUF + NSB * SB, LDS_BYTES = HELD > TURN ? HELD : TURN;
   static_assert(LDS_BYTES <= 160 * 1024, "shared memory of a unit");
   const int out_tiles = (a.n_out + 15) / 16, per = EPI == MM_EPI_GATED ? BNT / 2 : BNT;
   a.m_tiles = (a.M + BM - 1) / BM;
@@ -417,35 +461,46 @@ static int launch_mx4_many(Mx4ManyArgs a) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return LLM_ERR_LAUNCH;
   if (!asked[dev]) {
-    if (hipFuncSetAttribute((const void*)gemm_mx4_many_kernel<X4, WM, WN, MTW, NTW, EPI, OutT>,
+    if (hipFuncSetAttribute((const void*)gemm_mx4_many_kernel<X4, NBUF, WM, WN, MTW, NTW, EPI, OutT>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES) != hipSuccess)
       return LLM_ERR_LAUNCH;
     asked[dev] = true;
   }
-  gemm_mx4_many_kernel<X4, WM, WN, MTW, NTW, EPI, OutT><<<(unsigned)blocks, NW * 64, LDS_BYTES, a.stream>>>(a);
+  const dim3 grid((unsigned)blocks, (a.quads + a.slice_quads - 1) / a.slice_quads);
+  gemm_mx4_many_kernel<X4, NBUF, WM, WN, MTW, NTW, EPI, OutT><<<grid, NW * 64, LDS_BYTES, a.stream>>>(a);
   return llm_launch_status();
 }
 
+// Forms: rows of X by rows of W a block.
+#define MM_FORMS 4
 template <bool X4, int EPI, typename OutT>
-static int pick_mx4_many(const Mx4ManyArgs& a) {
-  return launch_mx4_many<X4, 2, 4, 8, 4, EPI, OutT>(a);
+static int pick_mx4_many(const Mx4ManyArgs& a, int form) {
+  switch (form) {
+    case 0: return launch_mx4_many<X4, 2, 2, 4, 8, 4, EPI, OutT>(a);             // 256 x 256
+    case 1: return launch_mx4_many<X4, 2, 4, 2, 4, 4, EPI, OutT>(a);             // 256 x 128
+    case 2: return launch_mx4_many<X4, X4 ? 4 : 2, 2, 2, 4, 4, EPI, OutT>(a);    // 128 x 128
+    case 3: return launch_mx4_many<X4, 4, 1, 4, 4, 2, EPI, OutT>(a);             // 64 x 128
+  }
+  return LLM_ERR_ARG;
 }
 
 template <bool X4>
-static int mx4_many(const Mx4ManyArgs& a, int epilogue, int out_dtype) {
-  if (epilogue == MM_EPI_GATED) return out_dtype == LLM_DTYPE_BF16 ? pick_mx4_many<X4, MM_EPI_GATED, bf16_t>(a) : LLM_ERR_ARG;
-  if (out_dtype == LLM_DTYPE_BF16) return pick_mx4_many<X4, MM_EPI_NONE, bf16_t>(a);
-  if (out_dtype == LLM_DTYPE_F32) return pick_mx4_many<X4, MM_EPI_NONE, float>(a);
+static int mx4_many(const Mx4ManyArgs& a, int epilogue, int out_dtype, int form) {
+  if (epilogue == MM_EPI_GATED) return out_dtype == LLM_DTYPE_BF16 ? pick_mx4_many<X4, MM_EPI_GATED, bf16_t>(a, form) : LLM_ERR_ARG;
+  if (out_dtype == LLM_DTYPE_BF16) return pick_mx4_many<X4, MM_EPI_NONE, bf16_t>(a, form);
+  if (out_dtype == LLM_DTYPE_F32) return pick_mx4_many<X4, MM_EPI_NONE, float>(a, form);
   return LLM_ERR_ARG;
 }
 
 // W [N, K] as mx4.h lays it out.  X: bfloat16 rows ldx apart with xs null (their length K and ldx
 // multiples of 128, what lies beyond W's width zero), or codes with their scales in xs.  epilogue 0:
 // C [M, N] of out_dtype, plus bias[n] if not null; 1 | act << 4: C [M, N / 2] in bfloat16, the gate
-// through an activation of common.h, N / 2 a multiple of 16.
+// through an activation of common.h, N / 2 a multiple of 16.  form: 0 .. 3, see above.  With k_split
+// above 1 (epilogue 0, float32, no bias) C is [k_split, M, N], the products over as many slices of K of
+// ceil(quads / k_split) quads of 512 elements; every slice has elements.
 extern "C" int llm_gemm_mx4_many(const void* X, const void* xs, int ldx, const void* wc, const void* ws,
                                  const float* bias, void* C, int epilogue, int out_dtype, int M, int N, int K,
-                                 hipStream_t stream) {
+                                 int form, int k_split, hipStream_t stream) {
   if (M <= 0) return LLM_OK;
   const int act = epilogue >> 4;
   epilogue &= 15;
@@ -471,5 +526,69 @@ extern "C" int llm_gemm_mx4_many(const void* X, const void* xs, int ldx, const v
   a.quads = mx4_quads(K);
   a.act = act;
   a.stream = stream;
-  return xs == nullptr ? mx4_many<false>(a, epilogue, out_dtype) : mx4_many<true>(a, epilogue, out_dtype);
+  if (k_split < 1 || form < 0 || form >= MM_FORMS) return LLM_ERR_ARG;
+  a.slice_quads = (a.quads + k_split - 1) / k_split;
+  if (k_split > 1 && (epilogue != MM_EPI_NONE || out_dtype != LLM_DTYPE_F32 || bias != nullptr ||
+                      (a.quads + a.slice_quads - 1) / a.slice_quads != k_split))
+    return LLM_ERR_ARG;
+  return xs == nullptr ? mx4_many<false>(a, epilogue, out_dtype, form) : mx4_many<true>(a, epilogue, out_dtype, form);
+}
+
+// The slices' sums parts [n_parts, M, N], added in their order, plus bias or through the gate, to C of
+// out_dtype: four columns a thread (N and n_out multiples of 4), or one.
+template <int VEC, bool GATED, typename OutT>
+__global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__ parts, int n_parts, const float* bias,
+                                                       OutT* __restrict__ C, size_t M, int N, int n_out, int act) {
+  const size_t i = (size_t)blockIdx.x * 256 + threadIdx.x;
+  const int per_row = n_out / VEC;
+  const size_t m = i / per_row;
+  const int n = (int)(i - m * per_row) * VEC;
+  if (m >= M) return;
+  float v[VEC], u[VEC];
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) v[e] = u[e] = 0.f;
+  for (int p = 0; p < n_parts; ++p) {
+    const float* src = parts + ((size_t)p * M + m) * N + n;
+    if constexpr (VEC == 4) {
+      const float4 q = *reinterpret_cast<const float4*>(src);
+      v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+      if (GATED) {
+        const float4 w = *reinterpret_cast<const float4*>(src + n_out);
+        u[0] += w.x; u[1] += w.y; u[2] += w.z; u[3] += w.w;
+      }
+    } else {
+      v[0] += src[0];
+      if (GATED) u[0] += src[n_out];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < VEC; ++e) {
+    if (GATED) v[e] = llm_gated(act, v[e], u[e]);
+    else if (bias != nullptr) v[e] += bias[n + e];
+  }
+  OutT* dst = C + m * n_out + n;
+  if constexpr (VEC == 4) Conv4<OutT>::store(dst, make_float4(v[0], v[1], v[2], v[3]));
+  else Conv<OutT>::store(dst, v[0]);
+}
+
+extern "C" int llm_mx4_join(const void* parts, int n_parts, const float* bias, void* C, int epilogue, int out_dtype,
+                            int M, int N, hipStream_t stream) {
+  if (M <= 0) return LLM_OK;
+  const int act = epilogue >> 4;
+  const bool gated = (epilogue & 15) == MM_EPI_GATED;
+  if (N <= 0 || n_parts <= 0 || act < 0 || act >= LLM_ACT_COUNT || parts == nullptr || C == nullptr || (gated && (N & 1))) return LLM_ERR_ARG;
+  const int n_out = gated ? N / 2 : N, vec = (n_out & 3) ? 1 : 4;
+  const size_t blocks = ((size_t)M * (n_out / vec) + 255) / 256;
+  if (blocks > 0x7fffffff) return LLM_ERR_ARG;
+#define MX4_JOIN(V, G, T) \
+  mx4_join_kernel<V, G, T><<<(unsigned)blocks, 256, 0, stream>>>((const float*)parts, n_parts, bias, (T*)C, M, N, n_out, act)
+#define MX4_JOIN_T(T)                                                 \
+  if (gated) { if (vec == 4) MX4_JOIN(4, true, T); else MX4_JOIN(1, true, T); } \
+  else { if (vec == 4) MX4_JOIN(4, false, T); else MX4_JOIN(1, false, T); }
+  if (out_dtype == LLM_DTYPE_BF16) { MX4_JOIN_T(bf16_t) }
+  else if (out_dtype == LLM_DTYPE_F32) { MX4_JOIN_T(float) }
+  else return LLM_ERR_ARG;
+#undef MX4_JOIN_T
+#undef MX4_JOIN
+  return llm_launch_status();
 }

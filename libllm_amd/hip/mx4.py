@@ -22,7 +22,8 @@ SIGNATURES = {
     "llm_mx4_pack": [_vp, _sz, _vp, _i, _i, _vp, _vp, _vp],
     "llm_pad_rows": [_vp, _sz, _vp, _i, _i, _i, _vp],
     "llm_gemm_mx4_rows": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
-    "llm_gemm_mx4_many": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "llm_gemm_mx4_many": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
+    "llm_mx4_join": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp],
 }
 
 
@@ -138,6 +139,17 @@ class Mx4Ops:
                     "pad_rows")
         return padded.data_ptr(), None, ldp, padded
 
+    _MX4_FORMS = ((256, 256), (256, 128), (128, 128), (64, 128))
+    mx4_force = None
+
+    def _mx4_form(self, m, n, k, epilogue, four):
+        if self.mx4_force:
+            form, ks = self.mx4_force
+            quads = -(-k // QUAD)
+            per = -(-quads // min(ks, quads))
+            return form, -(-quads // per)
+        return 0, 1
+
     def _mx4_product(self, x, w, out, epilogue, bias=None):
         from .ops import _code
         n, k = w.shape
@@ -145,14 +157,25 @@ class Mx4Ops:
         codes, scales = self._mx4(w, "MXFP4 weight")
         if m == 0:
             return out
-        many = m > self.MX4_ROWS
-        piece = 128 if many else 8
-        xp, xs, ldx, alive = self._mx4_rows(x, k, piece)
         bptr = None if bias is None else self._dev(bias, "bias", torch.float32, (n,))
-        # (where rows were padded, K is their padded length: the weight's codes there are zero)
-        fn = self.lib.llm_gemm_mx4_many if many else self.lib.llm_gemm_mx4_rows
-        self._check(fn(xp, xs, ldx, codes, scales, bptr, out.data_ptr(), epilogue, _code(out.dtype), m, n,
-                       -(-k // piece) * piece, self._stream()), "gemm_mx4_many" if many else "gemm_mx4_rows")
+        if m <= self.MX4_ROWS:
+            xp, xs, ldx, alive = self._mx4_rows(x, k, 8)
+            # (where rows were padded, K is their padded length: the weight's codes there are zero)
+            self._check(self.lib.llm_gemm_mx4_rows(xp, xs, ldx, codes, scales, bptr, out.data_ptr(), epilogue,
+                                                   _code(out.dtype), m, n, -(-k // 8) * 8, self._stream()), "gemm_mx4_rows")
+            return out
+        xp, xs, ldx, alive = self._mx4_rows(x, k, 128)
+        form, ks = self._mx4_form(m, n, k, epilogue, xs is not None)
+        kp = -(-k // 128) * 128
+        if ks == 1:
+            self._check(self.lib.llm_gemm_mx4_many(xp, xs, ldx, codes, scales, bptr, out.data_ptr(), epilogue,
+                                                   _code(out.dtype), m, n, kp, form, 1, self._stream()), "gemm_mx4_many")
+            return out
+        parts = torch.empty((ks, m, n), dtype=torch.float32, device=self.device)
+        self._check(self.lib.llm_gemm_mx4_many(xp, xs, ldx, codes, scales, None, parts.data_ptr(), self._EPI_NONE,
+                                               _code(torch.float32), m, n, kp, form, ks, self._stream()), "gemm_mx4_many")
+        self._check(self.lib.llm_mx4_join(parts.data_ptr(), ks, bptr, out.data_ptr(), epilogue, _code(out.dtype), m, n,
+                                          self._stream()), "mx4_join")
         return out
 
     def _linear_mx4(self, x, w, bias, out_dtype, residual=None):
