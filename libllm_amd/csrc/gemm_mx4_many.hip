@@ -18,8 +18,8 @@
 //
 // The fragments of a step are read into registers one step ahead of the matrix instructions that use
 // them, dealt out between those; the barrier of a tile lies in front of its last step, whose
-// fragments every wave has by then: behind it the loads of the tile after next go out into the
-// buffer that is left, and the first fragments of the next tile are read.
+// fragments every wave has by then: behind it the loads of a later tile go out into the buffer that
+// is left, and the first fragments of the next tile are read.
 #include "mx4.h"
 
 #include <type_traits>
@@ -70,6 +70,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   constexpr int BM = WM * MTW * 16, BNT = WN * NTW;         // rows of X, tiles of W a block
   constexpr int STEPS = X4 ? 2 : 4;
   constexpr int XB = X4 ? BM * 128 : BM * 256;              // bytes of X's tile of K
+  // With few waves a unit, nothing covers the latency of LDS: fragments are then read two steps ahead
+  // (into a second set) instead of one, and the barrier of a tile lies a step earlier.
+  constexpr bool EARLY = NBUF > 2;
+  // A buffer is then filled again a tile later than it could be: its reads are long over by then, and
+  // the barrier need not wait for those under way.
+  constexpr int AHEAD = EARLY ? 2 : 1, BSTEP = STEPS - AHEAD;
+  constexpr int FAR = EARLY ? NBUF - 1 : NBUF;              // tiles from the one at work to the one asked for
   constexpr bool WL = X4 || NBUF > 2;                       // W's codes and scales go through LDS
   constexpr int WB = X4 ? BNT * 2048 : WL ? BNT * 1024 : 0;
   constexpr int BUF = XB + WB;
@@ -185,7 +192,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   // its fragment of the next step is read into the same registers.  Addresses are kept few: the
   // compiler would hold one for every read of the loop and run out of registers.
   typedef uint32_t u4_raw __attribute__((ext_vector_type(4)));
-  Frag xf[MTW];
+  Frag xf[AHEAD][MTW];
   Frag wf[2][X4 ? NTW : 1];
   uint32_t sc[2][X4 ? (NTW + MTW) / 2 : 1];                 // scales of a tile of K: two bytes of two tiles a word
   u4_raw wc[2][X4 ? 1 : NTW];                               // W's codes of a tile of K, and its scales
@@ -235,7 +242,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     }
   };
 
-  each<NBUF>([&](auto b) MM_INLINE {
+  each<FAR>([&](auto b) MM_INLINE {
     if (b % TPQ == 0) fill_scales(b / TPQ);
     each<FILLS>([&](auto p) MM_INLINE { fill(b, b, p); });
   });
@@ -249,19 +256,30 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     load_w(0, 0);
     have_w(0);
   }
-  // What this wave asked for has arrived, but for the loads of that many tiles, the last ones.
-#define MM_ARRIVED(TILES) \
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(WL ? (TILES)*FILLS : 0) : "memory")
-  MM_ARRIVED(NBUF - 1);
-  __syncthreads();
-  {
-    const uint32_t x_at = x_step(0, 0);
+  // What this wave asked for has arrived, but for the loads of the last `tiles` tiles; then all waves.
+  auto arrived = [&](auto tiles) MM_INLINE {
+    constexpr int LEFT = WL ? decltype(tiles)::value * FILLS : 0;
+    if constexpr (EARLY) {
+      asm volatile("s_waitcnt vmcnt(%0)" : : "n"(LEFT) : "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    } else {
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(LEFT) : "memory");
+      __syncthreads();
+    }
+  };
+  arrived(std::integral_constant<int, FAR - 1>{});
 #pragma unroll
-    for (int mt = 0; mt < MTW; ++mt) xf[mt] = read_x(x_at, mt);
+  for (int ahead = 0; ahead < AHEAD; ++ahead) {
+    const uint32_t x_at = x_step(0, ahead);
+#pragma unroll
+    for (int mt = 0; mt < MTW; ++mt) xf[ahead][mt] = read_x(x_at, mt);
   }
   if constexpr (X4) {
 #pragma unroll
-    for (int nt = 0; nt < NTW; ++nt) wf[0][nt] = read_w(w_lane, nt);
+    for (int ahead = 0; ahead < AHEAD; ++ahead)
+#pragma unroll
+      for (int nt = 0; nt < NTW; ++nt) wf[ahead][nt] = read_w(w_lane + ahead * 1024, nt);
 #pragma unroll
     for (int i = 0; i < (NTW + MTW) / 2; ++i) {
       uint32_t lo, hi;
@@ -283,20 +301,20 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     if constexpr (!WL) load_w(min(kt + 1, n_kt - 1), NEXT);
     each<STEPS>([&](auto step) MM_INLINE {
       constexpr int S = decltype(step)::value, SET = S & 1;
-      constexpr bool LAST = S == STEPS - 1;
-      constexpr int RBUF = (TURN + LAST) % NBUF, RS = LAST ? 0 : S + 1;      // where the next step's fragments lie
-      if constexpr (LAST) {
+      constexpr int XS = EARLY ? SET : 0;
+      constexpr bool BORDER = S == BSTEP;                                    // from here on everything read is the next tile's
+      constexpr int RBUF = (TURN + (S >= BSTEP)) % NBUF, RS = (S + AHEAD) % STEPS;      // where the fragments to be read lie
+      if constexpr (BORDER) {
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!WL) have_w(NEXT);
-        MM_ARRIVED(NBUF - 2);
-        __syncthreads();
+        arrived(std::integral_constant<int, FAR - 2>{});
       }
       const uint32_t x_at = x_step(RBUF, RS);
       uint32_t w_at = 0, s_at = 0;
       Frag w[X4 ? 1 : NTW];
       if constexpr (WL) {
-        if constexpr (X4 || LAST) w_at = plus(w_lane, RBUF * BUF + (X4 ? RS * 1024 : 0));
-        if constexpr (LAST)
+        if constexpr (X4 || BORDER) w_at = plus(w_lane, RBUF * BUF + (X4 ? RS * 1024 : 0));
+        if constexpr (BORDER)
           s_at = plus(lane4, lds0 + NBUF * BUF + (((kt + 1) / TPQ) & (NSB - 1)) * SB + (TURN + 1) % TPQ * (X4 ? 2 : 1));
       }
       if constexpr (!X4) {
@@ -308,31 +326,36 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
         constexpr int MT = decltype(mtc)::value;
         __builtin_amdgcn_sched_barrier(0);
         // this group's share of the loads into the buffer that is left
-        if constexpr (LAST) {
-          if (MT == 0 && (TURN + NBUF) % TPQ == 0) fill_scales((kt + NBUF) / TPQ);
+        if constexpr (BORDER) {
+          if (MT == 0 && (TURN + FAR) % TPQ == 0) fill_scales((kt + FAR) / TPQ);
 #pragma unroll
-          for (int p = FILLS * MT / MTW; p < FILLS * (MT + 1) / MTW; ++p) fill(kt + NBUF, TURN % NBUF, p);
+          for (int p = FILLS * MT / MTW; p < FILLS * (MT + 1) / MTW; ++p) fill(kt + FAR, (TURN + FAR) % NBUF, p);
         }
         each<NTW>([&](auto ntc) MM_INLINE {
           constexpr int NT = decltype(ntc)::value;
           if constexpr (X4)
-            acc[NT][MT] = mx4_mfma<(NT & 1) * 2 + S, (MT & 1) * 2 + S>(wf[SET][NT].u, sc[CUR][NT / 2], xf[MT].u,
+            acc[NT][MT] = mx4_mfma<(NT & 1) * 2 + S, (MT & 1) * 2 + S>(wf[SET][NT].u, sc[CUR][NT / 2], xf[XS][MT].u,
                                                                        sc[CUR][NTW / 2 + MT / 2], acc[NT][MT]);
           else
-            acc[NT][MT] = mfma_bf16(w[NT], xf[MT], acc[NT][MT]);
+            acc[NT][MT] = mfma_bf16(w[NT], xf[XS][MT], acc[NT][MT]);
         });
         __builtin_amdgcn_sched_barrier(0);
-        // its share of the next step's reads, behind them
-        xf[MT] = read_x(x_at, MT);
+        // its share of the reads, behind them
+        xf[XS][MT] = read_x(x_at, MT);
         if constexpr (X4) {
+          if constexpr (!EARLY) {
 #pragma unroll
-          for (int nt = NTW * MT / MTW; nt < NTW * (MT + 1) / MTW; ++nt) wf[SET ^ 1][nt] = read_w(w_at, nt);
-          if constexpr (LAST) {
+            for (int nt = NTW * MT / MTW; nt < NTW * (MT + 1) / MTW; ++nt) wf[SET ^ 1][nt] = read_w(w_at, nt);
+          } else if constexpr (MT == MTW - 1) {              // (this step's are done with)
+#pragma unroll
+            for (int nt = 0; nt < NTW; ++nt) wf[SET][nt] = read_w(w_at, nt);
+          }
+          if constexpr (BORDER) {
             constexpr int NS = (NTW + MTW) / 2;
 #pragma unroll
             for (int i = NS * MT / MTW; i < NS * (MT + 1) / MTW; ++i) read_scales(s_at, i, sc_lo[i], sc_hi[i]);
           }
-        } else if constexpr (WL && LAST) {
+        } else if constexpr (WL && BORDER) {
 #pragma unroll
           for (int nt = NTW * MT / MTW; nt < NTW * (MT + 1) / MTW; ++nt) {
             wc[NEXT][nt] = read_codes(w_at, nt);
@@ -471,15 +494,24 @@ static int launch_mx4_many(Mx4ManyArgs a) {
   return llm_launch_status();
 }
 
-// Forms: rows of X by rows of W a block.
+// Forms: rows of X by rows of W a block.  0, 256 x 256: fewest bytes a product, one block a unit.  1,
+// 128 x 128 (MXFP4 rows only: in bfloat16 form 2 is as fast or faster at every size measured).  2,
+// 64 x 128: several blocks a unit, which cover each other's waits.  3, 64 x 128 with four tiles of K
+// held and fragments two steps ahead: for a block a unit or less, where a block waits for memory (1.5 us
+// from a weight that no cache holds).  In bfloat16 that form has eight waves (128 rows, K 4,096, 6,144
+// outputs, us: 19.6, by four waves 22.3, form 2 27.5).
 #define MM_FORMS 4
 template <bool X4, int EPI, typename OutT>
 static int pick_mx4_many(const Mx4ManyArgs& a, int form) {
   switch (form) {
-    case 0: return launch_mx4_many<X4, 2, 2, 4, 8, 4, EPI, OutT>(a);             // 256 x 256
-    case 1: return launch_mx4_many<X4, 2, 4, 2, 4, 4, EPI, OutT>(a);             // 256 x 128
-    case 2: return launch_mx4_many<X4, X4 ? 4 : 2, 2, 2, 4, 4, EPI, OutT>(a);    // 128 x 128
-    case 3: return launch_mx4_many<X4, 4, 1, 4, 4, 2, EPI, OutT>(a);             // 64 x 128
+    case 0: return launch_mx4_many<X4, 2, 2, 4, 8, 4, EPI, OutT>(a);
+    case 1:
+      if constexpr (X4) return launch_mx4_many<X4, 2, 2, 2, 4, 4, EPI, OutT>(a);
+      break;
+    case 2: return launch_mx4_many<X4, 2, 1, 4, 4, 2, EPI, OutT>(a);
+    case 3:
+      if constexpr (X4) return launch_mx4_many<X4, 4, 1, 4, 4, 2, EPI, OutT>(a);
+      else return launch_mx4_many<X4, 4, 2, 4, 2, 2, EPI, OutT>(a);
   }
   return LLM_ERR_ARG;
 }

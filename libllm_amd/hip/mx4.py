@@ -13,8 +13,8 @@ from ..errors import KernelError
 
 _vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
 
-BLOCK = 32              # elements that share a scale
-TILE_ROWS, QUAD = 16, 512      # a tile holds 16 rows by whole quads of 512 elements
+BLOCK = 32                      # elements that share a scale
+TILE_ROWS, QUAD = 16, 512       # a tile holds 16 rows by whole quads of 512 elements
 
 SIGNATURES = {
     "llm_mx4_quantize": [_vp, _i, _sz, _i, _i, _vp, _vp, _vp],
@@ -29,22 +29,26 @@ SIGNATURES = {
 
 def tiled_sizes(rows: int, width: int):
     """(bytes of codes, bytes of scales) of a matrix of these sizes, whole tiles."""
-    tiles, quads = -(-rows // TILE_ROWS), -(-width // QUAD)
-    return tiles * quads * 4096, tiles * quads * 256
+    cells = -(-rows // TILE_ROWS) * -(-width // QUAD)
+    return cells * 4096, cells * 256
 
 
 class Mx4Matrix:
-    """A matrix ``[rows, width]`` in MXFP4: ``codes`` and ``scales`` are uint8 tensors in the order
-    the matrix cores read them.  What ``HipOps.quantize_mx4`` and ``HipOps.mx4_from_codes`` return, and the
-    products take as a weight, or on both sides."""
+    """A matrix ``[rows, width]`` in MXFP4: ``codes`` and ``scales`` are flat uint8 tensors in the
+    order the matrix cores read them.  What ``HipOps.quantize_mx4`` and ``HipOps.mx4_from_codes``
+    return, and the products take as a weight, or on both sides."""
     dtype = "mxfp4"
 
     def __init__(self, shape, codes, scales):
-        self.shape, self.codes, self.scales = tuple(shape), codes, scales
-
-    @property
-    def device(self):
-        return self.codes.device
+        rows, width = shape
+        want = tiled_sizes(rows, width)
+        for t, size, what in ((codes, want[0], "codes"), (scales, want[1], "scales")):
+            if t.dtype != torch.uint8 or tuple(t.shape) != (size,) or not t.is_contiguous() or t.data_ptr() % 16:
+                raise KernelError("the %s of an MXFP4 matrix [%d, %d] are %d bytes in a row, 16-byte aligned"
+                                  % (what, rows, width, size))
+        if codes.device != scales.device:
+            raise KernelError("codes and scales of an MXFP4 matrix lie on %s and %s" % (codes.device, scales.device))
+        self.shape, self.codes, self.scales, self.device = (rows, width), codes, scales, codes.device
 
     def leading_rows(self, rows: int) -> "Mx4Matrix":
         """The first ``rows`` rows, a multiple of 16, in the same storage."""
@@ -58,45 +62,45 @@ class Mx4Matrix:
 class Mx4Ops:
     """The operations of ``HipOps`` on matrices in MXFP4."""
 
-    MX4_ROWS = 32           # most rows that go to the product for few rows
+    MX4_ROWS = 32           # most rows that go to the product for few rows wherever W goes
+    MX4_PLANS = 4096        # launch plans kept, by sizes
 
+    # ---- conversions
     def _mx4_empty(self, rows, width):
         if rows <= 0 or width <= 0:
             raise KernelError("an MXFP4 matrix has rows and columns, not [%d, %d]" % (rows, width))
         if max(rows, width) >= 1 << 30:
             raise KernelError("an MXFP4 matrix of [%d, %d] is too large" % (rows, width))
         codes, scales = tiled_sizes(rows, width)
-        return Mx4Matrix((rows, width), torch.empty(codes, dtype=torch.uint8, device=self.device),
-                         torch.empty(scales, dtype=torch.uint8, device=self.device))
+        both = torch.empty(codes + scales, dtype=torch.uint8, device=self.device)
+        return Mx4Matrix((rows, width), both[:codes], both[codes:])
 
     def _mx4(self, q, what):
-        """Checks a matrix in MXFP4; returns the pointers to its codes and scales."""
         if not isinstance(q, Mx4Matrix):
             raise KernelError("%s is no MXFP4 matrix" % what)
-        codes, scales = tiled_sizes(*q.shape)
-        return (self._dev(q.codes, what + " codes", torch.uint8, (codes,)),
-                self._dev(q.scales, what + " scales", torch.uint8, (scales,)))
+        if q.device != self.device:
+            raise KernelError("%s lies on %s, not on %s" % (what, q.device, self.device))
+        return q
 
     def quantize_mx4(self, x) -> Mx4Matrix:
         """The matrix ``x`` (bfloat16 or float32, rows contiguous; they may lie further apart than
         their length) in MXFP4.  The scale of a block is 2^(floor(log2(max |x|)) - 2), at least
         2^-127; an element is divided by it and rounded to the nearest code, ties to the even one,
         6 beyond 6.  A block that holds an infinity or a NaN reads as NaN."""
-        from .ops import _code
-        self._weight(x, "the matrix to quantise")
-        q = self._mx4_empty(*x.shape)
-        self._check(self.lib.llm_mx4_quantize(
-            x.data_ptr(), _code(x.dtype), max(x.stride(0), x.shape[1]), x.shape[0], x.shape[1], q.codes.data_ptr(), q.scales.data_ptr(),
-            self._stream()), "quantize_mx4")
+        self._matrix(x, "the matrix to quantise")
+        m, k = x.shape
+        q = self._mx4_empty(m, k)
+        self._launch("llm_mx4_quantize", x.data_ptr(), self._dtype_code(x.dtype), max(x.stride(0), k), m, k,
+                     q.codes.data_ptr(), q.scales.data_ptr())
         return q
 
     def dequantize_mx4(self, q: Mx4Matrix, dtype=torch.bfloat16) -> torch.Tensor:
         """The numbers that ``q`` stands for, exactly (a scale above 2^125 can give an infinity)."""
-        from .ops import _code
-        codes, scales = self._mx4(q, "the matrix to read")
-        out = torch.empty(q.shape, dtype=dtype, device=self.device)
-        self._check(self.lib.llm_mx4_dequantize(codes, scales, out.data_ptr(), _code(dtype), q.shape[0], q.shape[1],
-                                                self._stream()), "dequantize_mx4")
+        self._mx4(q, "the matrix to read")
+        code = self._dtype_code(dtype)
+        m, k = q.shape
+        out = torch.empty((m, k), dtype=dtype, device=self.device)
+        self._launch("llm_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), code, m, k)
         return out
 
     def mx4_from_codes(self, codes, scales, width=None) -> Mx4Matrix:
@@ -104,110 +108,146 @@ class Mx4Ops:
         ``[rows, ceil(width / 2)]`` or wider, two elements a byte, the even one in the low half, and
         ``scales`` uint8 ``[rows, ceil(width / 32)]``.  ``width``: twice the columns of ``codes``
         unless it is given (an odd width, padded rows)."""
-        if codes.dim() != 2 or codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise KernelError("mx4_from_codes: codes and scales are matrices of uint8")
-        self._weight(codes, "the matrix of codes")
+        self._matrix(codes, "the matrix of codes")
         rows, columns = codes.shape
         width = 2 * columns if width is None else int(width)
         if not 0 < -(-width // 2) <= columns:
             raise KernelError("mx4_from_codes: %d columns of codes do not hold rows of %d elements" % (columns, width))
         self._dev(scales, "the matrix of scales", torch.uint8, (rows, -(-width // BLOCK)))
         q = self._mx4_empty(rows, width)
-        self._check(self.lib.llm_mx4_pack(codes.data_ptr(), max(codes.stride(0), columns), scales.data_ptr(), rows, width,
-                                          q.codes.data_ptr(), q.scales.data_ptr(), self._stream()), "mx4_from_codes")
+        self._launch("llm_mx4_pack", codes.data_ptr(), max(codes.stride(0), columns), scales.data_ptr(), rows, width,
+                     q.codes.data_ptr(), q.scales.data_ptr())
         return q
 
-    def _mx4_rows(self, x, k, piece):
-        """Rows for a product with an MXFP4 weight that reads ``piece`` elements of them at a time:
-        (pointer, pointer to scales or None, row stride, what keeps them alive).  bfloat16 rows
-        whose length, distance or address does not allow that are copied to a padded buffer first."""
-        if isinstance(x, Mx4Matrix):
-            codes, scales = self._mx4(x, "linear input")
-            return codes, scales, 0, x
+    def _matrix(self, x, what):
+        """A matrix on the device with contiguous rows."""
         if x.device != self.device:
-            raise KernelError("linear input lies on %s, not on %s" % (x.device, self.device))
+            raise KernelError("%s lies on %s, not on %s" % (what, x.device, self.device))
+        if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
+            raise KernelError("%s must be a matrix with contiguous rows" % what)
+
+    # ---- products
+    def _mx4_few(self, m, n_out, four):
+        """Whether the product goes to the kernel for few rows: up to MX4_ROWS, and up to twice as many
+        where W has few tiles of outputs, so that the other would leave units idle (us, 64 rows,
+        that kernel against this: bfloat16, K 2,048, 2,048 outputs 5.5 against 10.4, but K 4,096,
+        6,144 outputs 17.5 against 17.8 and K 14,336, 4,096 outputs 36 against 22; MXFP4, in the
+        same order, 3.6 against 6.2, 8.6 against 11.1 and 18.3 against 17.5)."""
+        tiles = -(-n_out // TILE_ROWS)
+        return m <= self.MX4_ROWS or (m <= 2 * self.MX4_ROWS and 2 * tiles <= (3 if four else 1) * self.units)
+
+    # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, and the us
+    # that 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much
+    # again for every four).  Measured over 2,048 to 14,336 elements of K, 33 to 4,096 rows, 2,048 to
+    # 28,672 outputs; the forms' times cross where this says within a tenth.
+    _MX4_FORMS = {
+        False: ((0, 256, 256, (2.7, 5.4, 8.1, 10.8)), (2, 64, 128, (0.71, 1.0, 1.43, 1.75)),
+                (3, 64, 128, (0.58, 1.15, 1.75, 2.3))),
+        True: ((0, 256, 256, (0.94, 1.88, 2.82, 3.76)), (1, 128, 128, (0.49, 0.63, 1.14, 1.33)),
+               (2, 64, 128, (0.38, 0.44, 0.72, 0.85)), (3, 64, 128, (0.26, 0.52, 0.78, 1.04))),
+    }
+
+    def _mx4_form(self, m, n, k, four):
+        """(form, slices of K) of the product for many rows: those for which blocks, times and the
+        adding of the slices (each written and read in 32 bits, and a launch) come out lowest."""
+        quads, all_units = -(-k // QUAD), -(-k // 128)
+        best = None
+        for form, rows, cols, times in self._MX4_FORMS[four]:
+            blocks = -(-m // rows) * -(-n // cols)
+            for ks in (1, 2, 4, 8, 16):
+                if ks > quads or (ks > 1 and blocks * ks > 2 * self.units):
+                    break
+                per = -(-quads // ks)
+                if -(-quads // per) != ks:
+                    continue
+                a_unit = -(-blocks * ks // self.units)
+                cost = min(4 * per, all_units) * (times[3] * ((a_unit - 1) // 4) + times[(a_unit - 1) % 4])
+                if ks > 1:
+                    cost += 3.0 + ks * m * n * 8 / 4e6
+                if best is None or cost < best[0]:
+                    best = (cost, form, ks)
+        return best[1:]
+
+    def _mx4_plan(self, m, n, n_out, k, four):
+        """(form, slices of K), form -1 being the kernel for few rows.  Kept by sizes: choosing takes
+        longer than a small product."""
+        key = (m, n, n_out, k, four)
+        plan = self._mx4_plans.get(key)
+        if plan is None:
+            if len(self._mx4_plans) >= self.MX4_PLANS:
+                self._mx4_plans.clear()
+            plan = (-1, 1) if self._mx4_few(m, n_out, four) else self._mx4_form(m, n, k, four)
+            self._mx4_plans[key] = plan
+        return plan
+
+    def _mx4_rows(self, x, k, piece):
+        """bfloat16 rows for a kernel that reads ``piece`` elements of them at a time: ``x`` itself, or a
+        padded copy where its length, distance or address does not allow that."""
         if x.dtype != torch.bfloat16:
             raise KernelError("linear: an MXFP4 weight takes rows in bfloat16 or MXFP4, not %s" % (x.dtype,))
-        if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < k):
-            raise KernelError("linear input must be a matrix with contiguous rows")
+        self._matrix(x, "linear input")
         ld = max(x.stride(0), k)
         if k % piece == 0 and ld % piece == 0 and x.data_ptr() % 16 == 0:
-            return x.data_ptr(), None, ld, x
+            return x, ld
         ldp = -(-k // piece) * piece
         padded = torch.empty((x.shape[0], ldp), dtype=torch.bfloat16, device=self.device)
-        self._check(self.lib.llm_pad_rows(x.data_ptr(), ld, padded.data_ptr(), x.shape[0], k, ldp, self._stream()),
-                    "pad_rows")
-        return padded.data_ptr(), None, ldp, padded
+        self._launch("llm_pad_rows", x.data_ptr(), ld, padded.data_ptr(), x.shape[0], k, ldp)
+        return padded, ldp
 
-    _MX4_FORMS = ((256, 256), (256, 128), (128, 128), (64, 128))
-    mx4_force = None
-
-    def _mx4_form(self, m, n, k, epilogue, four):
-        if self.mx4_force:
-            form, ks = self.mx4_force
-            quads = -(-k // QUAD)
-            per = -(-quads // min(ks, quads))
-            return form, -(-quads // per)
-        return 0, 1
-
-    def _mx4_product(self, x, w, out, epilogue, bias=None):
-        from .ops import _code
+    def _mx4_product(self, x, w, n_out, out_dtype, epilogue, bias=None):
+        self._mx4(w, "the weight")
         n, k = w.shape
-        m = out.shape[0]
-        codes, scales = self._mx4(w, "MXFP4 weight")
+        m, k2 = x.shape
+        if k != k2:
+            raise KernelError("linear: x is [%d, %d] but the weight is [%d, %d]" % (m, k2, n, k))
+        code = self._dtype_code(out_dtype)
+        bptr = None if bias is None else self._dev(bias, "bias", torch.float32, (n,))
+        out = torch.empty((m, n_out), dtype=out_dtype, device=self.device)
         if m == 0:
             return out
-        bptr = None if bias is None else self._dev(bias, "bias", torch.float32, (n,))
-        if m <= self.MX4_ROWS:
-            xp, xs, ldx, alive = self._mx4_rows(x, k, 8)
-            # (where rows were padded, K is their padded length: the weight's codes there are zero)
-            self._check(self.lib.llm_gemm_mx4_rows(xp, xs, ldx, codes, scales, bptr, out.data_ptr(), epilogue,
-                                                   _code(out.dtype), m, n, -(-k // 8) * 8, self._stream()), "gemm_mx4_rows")
-            return out
-        xp, xs, ldx, alive = self._mx4_rows(x, k, 128)
-        form, ks = self._mx4_form(m, n, k, epilogue, xs is not None)
-        kp = -(-k // 128) * 128
-        if ks == 1:
-            self._check(self.lib.llm_gemm_mx4_many(xp, xs, ldx, codes, scales, bptr, out.data_ptr(), epilogue,
-                                                   _code(out.dtype), m, n, kp, form, 1, self._stream()), "gemm_mx4_many")
-            return out
-        parts = torch.empty((ks, m, n), dtype=torch.float32, device=self.device)
-        self._check(self.lib.llm_gemm_mx4_many(xp, xs, ldx, codes, scales, None, parts.data_ptr(), self._EPI_NONE,
-                                               _code(torch.float32), m, n, kp, form, ks, self._stream()), "gemm_mx4_many")
-        self._check(self.lib.llm_mx4_join(parts.data_ptr(), ks, bptr, out.data_ptr(), epilogue, _code(out.dtype), m, n,
-                                          self._stream()), "mx4_join")
+        four = isinstance(x, Mx4Matrix)
+        form, ks = self._mx4_plan(m, n, n_out, k, four)
+        piece = 8 if form < 0 else 128
+        if four:
+            self._mx4(x, "linear input")
+            xp, xs, ldx = x.codes.data_ptr(), x.scales.data_ptr(), 0
+        else:
+            x, ldx = self._mx4_rows(x, k, piece)
+            xp, xs = x.data_ptr(), None
+        kp = -(-k // piece) * piece         # (where rows were padded, their length: the weight's codes there are zero)
+        wp, ws = w.codes.data_ptr(), w.scales.data_ptr()
+        if form < 0:
+            self._launch("llm_gemm_mx4_rows", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp)
+        elif ks == 1:
+            self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp, form, 1)
+        else:
+            parts = torch.empty((ks, m, n), dtype=torch.float32, device=self.device)
+            self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, None, parts.data_ptr(), self._EPI_NONE,
+                         self._dtype_code(torch.float32), m, n, kp, form, ks)
+            self._launch("llm_mx4_join", parts.data_ptr(), ks, bptr, out.data_ptr(), epilogue, code, m, n)
         return out
 
     def _linear_mx4(self, x, w, bias, out_dtype, residual=None):
         """``linear`` with an MXFP4 weight.  With ``residual`` the product is returned, for the norm
         that comes next to add."""
-        from .ops import NormedRows
-        if isinstance(x, NormedRows):
-            x = self._materialise(x, torch.bfloat16)
-        m, k = x.shape
-        n = w.shape[0]
-        if k != w.shape[1]:
-            raise KernelError("linear: x is [%d, %d] but the weight is [%d, %d]" % (m, k, n, w.shape[1]))
-        return self._mx4_product(x, w, torch.empty((m, n), dtype=out_dtype, device=self.device), self._EPI_NONE, bias)
+        x = self._materialise(x, torch.bfloat16)
+        return self._mx4_product(x, w, w.shape[0], out_dtype, self._EPI_NONE, bias)
 
     def _linear_swiglu_mx4(self, x, w, dtype, activation):
         """The gated product with a stacked MXFP4 weight.  Gate and up stay in 32 bits until the
         result is rounded."""
-        from .ops import NormedRows
-        if isinstance(x, NormedRows):
-            x = self._materialise(x, torch.bfloat16)
-        if dtype is None:
-            dtype = torch.bfloat16
-        m, k = x.shape
+        x = self._materialise(x, torch.bfloat16)
         act = self._act(activation)
-        if w.shape[0] % 2:
+        dtype = dtype or torch.bfloat16
+        n = w.shape[0]
+        if n % 2:
             raise KernelError("linear_swiglu: the stacked weight has an odd number of rows")
-        if k != w.shape[1]:
-            raise KernelError("linear_swiglu: x is [%d, %d] but the weight is %s" % (m, k, w.shape))
-        inter = w.shape[0] // 2
-        if dtype == torch.bfloat16 and inter % TILE_ROWS == 0:
-            out = torch.empty((m, inter), dtype=torch.bfloat16, device=self.device)
-            return self._mx4_product(x, w, out, self._EPI_SWIGLU | (act << 4))
+        if dtype == torch.bfloat16 and n // 2 % TILE_ROWS == 0:
+            return self._mx4_product(x, w, n // 2, dtype, self._EPI_SWIGLU | (act << 4))
         # up's rows begin inside a tile, or the result is wanted in 32 bits: the product in 32 bits, then the gate
-        out = self.silu_mul(self._linear_mx4(x, w, None, torch.float32), activation)
+        if x.shape[0] == 0:
+            return torch.empty((0, n // 2), dtype=dtype, device=self.device)
+        out = self.silu_mul(self._mx4_product(x, w, n, torch.float32, self._EPI_NONE), activation)
         return out if out.dtype == dtype else out.to(dtype)

@@ -177,6 +177,8 @@ class HipOps(Mx4Ops):
         self.device = torch.device(device or "cuda:0")
         if self.device.type != "cuda":
             raise KernelError("device %s is not a GPU" % (self.device,))
+        self._index = torch.cuda.current_device() if self.device.index is None else self.device.index
+        self._mx4_plans = {}            # sizes of a product with an MXFP4 weight -> how it is launched
         self.lib = build.load()
         for name, argtypes in _SIGNATURES.items():
             try:
@@ -252,6 +254,24 @@ class HipOps(Mx4Ops):
     # ---- helpers
     def _stream(self):
         return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _launch(self, name, *args):
+        """Calls the entry point ``name`` on the current stream of this object's device, whichever
+        device is the current one."""
+        index = self._index
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        fn = getattr(self.lib, name)
+        if torch._C._cuda_getDevice() == index:
+            status = fn(*args, stream)
+        else:
+            with torch.cuda.device(index):
+                status = fn(*args, stream)
+        if status != 0:
+            self._check(status, name[4:])
+
+    @staticmethod
+    def _dtype_code(dtype):
+        return _code(dtype)
 
     @staticmethod
     def _check(status: int, what: str):
