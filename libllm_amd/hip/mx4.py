@@ -38,6 +38,7 @@ class Mx4Matrix:
     order the matrix cores read them.  What ``HipOps.quantize_mx4`` and ``HipOps.mx4_from_codes``
     return, and the products take as a weight, or on both sides."""
     dtype = "mxfp4"
+    __slots__ = ("shape", "device", "codes_ptr", "scales_ptr", "_storage")
 
     def __init__(self, shape, codes, scales):
         rows, width = shape
@@ -48,7 +49,33 @@ class Mx4Matrix:
                                   % (what, rows, width, size))
         if codes.device != scales.device:
             raise KernelError("codes and scales of an MXFP4 matrix lie on %s and %s" % (codes.device, scales.device))
-        self.shape, self.codes, self.scales, self.device = (rows, width), codes, scales, codes.device
+        self.shape, self.device, self._storage = (rows, width), codes.device, (codes, scales)
+        self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
+
+    @classmethod
+    def _new(cls, rows, width, device):
+        """Room for a matrix: one allocation, the codes first."""
+        q = cls.__new__(cls)
+        codes, scales = tiled_sizes(rows, width)
+        both = torch.empty(codes + scales, dtype=torch.uint8, device=device)
+        q.shape, q.device, q._storage = (rows, width), device, both
+        q.codes_ptr = both.data_ptr()
+        q.scales_ptr = q.codes_ptr + codes
+        return q
+
+    @property
+    def codes(self):
+        return self._parts()[0]
+
+    @property
+    def scales(self):
+        return self._parts()[1]
+
+    def _parts(self):
+        if not isinstance(self._storage, tuple):
+            size = tiled_sizes(*self.shape)[0]
+            self._storage = (self._storage[:size], self._storage[size:])
+        return self._storage
 
     def leading_rows(self, rows: int) -> "Mx4Matrix":
         """The first ``rows`` rows, a multiple of 16, in the same storage."""
@@ -69,11 +96,9 @@ class Mx4Ops:
     def _mx4_empty(self, rows, width):
         if rows <= 0 or width <= 0:
             raise KernelError("an MXFP4 matrix has rows and columns, not [%d, %d]" % (rows, width))
-        if max(rows, width) >= 1 << 30:
+        if rows >= 1 << 30 or width > 65535 * QUAD:
             raise KernelError("an MXFP4 matrix of [%d, %d] is too large" % (rows, width))
-        codes, scales = tiled_sizes(rows, width)
-        both = torch.empty(codes + scales, dtype=torch.uint8, device=self.device)
-        return Mx4Matrix((rows, width), both[:codes], both[codes:])
+        return Mx4Matrix._new(rows, width, self.device)
 
     def _mx4(self, q, what):
         if not isinstance(q, Mx4Matrix):
@@ -91,7 +116,7 @@ class Mx4Ops:
         m, k = x.shape
         q = self._mx4_empty(m, k)
         self._launch("llm_mx4_quantize", x.data_ptr(), self._dtype_code(x.dtype), max(x.stride(0), k), m, k,
-                     q.codes.data_ptr(), q.scales.data_ptr())
+                     q.codes_ptr, q.scales_ptr)
         return q
 
     def dequantize_mx4(self, q: Mx4Matrix, dtype=torch.bfloat16) -> torch.Tensor:
@@ -100,7 +125,7 @@ class Mx4Ops:
         code = self._dtype_code(dtype)
         m, k = q.shape
         out = torch.empty((m, k), dtype=dtype, device=self.device)
-        self._launch("llm_mx4_dequantize", q.codes.data_ptr(), q.scales.data_ptr(), out.data_ptr(), code, m, k)
+        self._launch("llm_mx4_dequantize", q.codes_ptr, q.scales_ptr, out.data_ptr(), code, m, k)
         return out
 
     def mx4_from_codes(self, codes, scales, width=None) -> Mx4Matrix:
@@ -118,7 +143,7 @@ class Mx4Ops:
         self._dev(scales, "the matrix of scales", torch.uint8, (rows, -(-width // BLOCK)))
         q = self._mx4_empty(rows, width)
         self._launch("llm_mx4_pack", codes.data_ptr(), max(codes.stride(0), columns), scales.data_ptr(), rows, width,
-                     q.codes.data_ptr(), q.scales.data_ptr())
+                     q.codes_ptr, q.scales_ptr)
         return q
 
     def _matrix(self, x, what):
@@ -185,15 +210,19 @@ class Mx4Ops:
     def _mx4_rows(self, x, k, piece):
         """bfloat16 rows for a kernel that reads ``piece`` elements of them at a time: ``x`` itself, or a
         padded copy where its length, distance or address does not allow that."""
+        at = x.data_ptr()
+        if (x.dtype is torch.bfloat16 and x.device == self.device and x.dim() == 2 and x.is_contiguous()
+                and k % piece == 0 and at % 16 == 0):
+            return x, k
         if x.dtype != torch.bfloat16:
             raise KernelError("linear: an MXFP4 weight takes rows in bfloat16 or MXFP4, not %s" % (x.dtype,))
         self._matrix(x, "linear input")
         ld = max(x.stride(0), k)
-        if k % piece == 0 and ld % piece == 0 and x.data_ptr() % 16 == 0:
+        if k % piece == 0 and ld % piece == 0 and at % 16 == 0:
             return x, ld
         ldp = -(-k // piece) * piece
         padded = torch.empty((x.shape[0], ldp), dtype=torch.bfloat16, device=self.device)
-        self._launch("llm_pad_rows", x.data_ptr(), ld, padded.data_ptr(), x.shape[0], k, ldp)
+        self._launch("llm_pad_rows", at, ld, padded.data_ptr(), x.shape[0], k, ldp)
         return padded, ldp
 
     def _mx4_product(self, x, w, n_out, out_dtype, epilogue, bias=None):
@@ -212,12 +241,12 @@ class Mx4Ops:
         piece = 8 if form < 0 else 128
         if four:
             self._mx4(x, "linear input")
-            xp, xs, ldx = x.codes.data_ptr(), x.scales.data_ptr(), 0
+            xp, xs, ldx = x.codes_ptr, x.scales_ptr, 0
         else:
             x, ldx = self._mx4_rows(x, k, piece)
             xp, xs = x.data_ptr(), None
         kp = -(-k // piece) * piece         # (where rows were padded, their length: the weight's codes there are zero)
-        wp, ws = w.codes.data_ptr(), w.scales.data_ptr()
+        wp, ws = w.codes_ptr, w.scales_ptr
         if form < 0:
             self._launch("llm_gemm_mx4_rows", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp)
         elif ks == 1:
