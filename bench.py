@@ -73,13 +73,15 @@ def log(msg):
     print("[bench] " + msg, file=sys.stderr, flush=True)
 
 
-def weight_bytes(cfg, itemsize):
+def weight_bytes(cfg, itemsize, weights="stored"):
     """Bytes of every weight a decode step reads once (the tied table serves as output matrix)."""
     h, i = cfg.hidden_size, cfg.intermediate_size
     q, kv = cfg.num_attention_heads * cfg.head_dim, cfg.num_key_value_heads * cfg.head_dim
     per_layer = (q + 2 * kv) * h + h * q + 3 * h * i
     head = cfg.vocab_size * h
     norms = (2 * cfg.num_hidden_layers + 1) * h * 4
+    if weights == "mxfp4":                                # 32 elements are 16 bytes and a scale
+        return cfg.num_hidden_layers * per_layer * 17 // 32 + head * itemsize + norms
     return (cfg.num_hidden_layers * per_layer + head) * itemsize + norms
 
 
@@ -424,6 +426,8 @@ def main() -> int:
     ap.add_argument("--context", type=int, default=4096)
     ap.add_argument("--prefill", type=int, default=2048)
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--weights", default="stored", choices=["stored", "mxfp4"],
+                    help="the layers' matrices in the dtype, or in microscaled 4-bit floating point (without --workload, --sweep, --unequal, --requests)")
     ap.add_argument("--no-points", action="store_true", help="skip decoding at batch 1, 64 and 256")
     ap.add_argument("--sampling", default="greedy", choices=["greedy", "default"],
                     help="greedy, or the command line's default (temperature 1, top-k 50, top-p 0.8)")
@@ -476,7 +480,7 @@ def main() -> int:
     max_tokens = biggest * (args.context + 64) + 4096
     log("building %d layers of %d with random weights, cache for %d tokens" %
         (args.layers, layers_full, max_tokens))
-    engine = random_engine(cfg, seed=0, dtype=args.dtype, max_tokens=max_tokens)
+    engine = random_engine(cfg, seed=0, dtype=args.dtype, max_tokens=max_tokens, weights=args.weights)
     gen = Generator(engine, Sampler(engine.ops, cfg.vocab_size), (), cfg.max_position_embeddings,
                     engine.cache.n_pages, PAGE, max_batch=biggest)
     params = SamplingParams(temperature=0.0) if args.sampling == "greedy" else SamplingParams()
@@ -494,7 +498,7 @@ def main() -> int:
     value = args.batch * args.steps / dt
     log("decode at batch %d: %.3f ms a step, %.0f tokens/s" % (args.batch, ms, value))
     mean_ctx = args.context - args.steps / 2.0
-    step_bytes = weight_bytes(cfg, itemsize) + args.batch * mean_ctx * kv_bytes_per_token(cfg, itemsize)
+    step_bytes = weight_bytes(cfg, itemsize, args.weights) + args.batch * mean_ctx * kv_bytes_per_token(cfg, itemsize)
     achieved = step_bytes / (dt / args.steps) / 1e9
 
     flops_measured = (peaks["bf16_TFs"] if short == "bf16" else peaks["fp32_TFs"]) * 1e12
@@ -503,7 +507,7 @@ def main() -> int:
         for b in point_batches:
             dtb = time_decode(gen, params, torch, b, args.context, args.steps, args.warmup, vocab)
             points["decode_b%d" % b] = round(b * args.steps / dtb, 1)
-            bytes_b = weight_bytes(cfg, itemsize) + b * mean_ctx * kv_bytes_per_token(cfg, itemsize)
+            bytes_b = weight_bytes(cfg, itemsize, args.weights) + b * mean_ctx * kv_bytes_per_token(cfg, itemsize)
             points["decode_b%d_hbm_frac" % b] = round(bytes_b / (dtb / args.steps) / HBM_BYTES_PER_S, 4)
             log("decode at batch %d: %.3f ms a step, %.0f tokens/s" % (b, dtb / args.steps * 1e3, b * args.steps / dtb))
     if 256 in point_batches:
@@ -513,9 +517,10 @@ def main() -> int:
         dtu = time_contexts(engine, torch, "unequal64", ctxs, 32, 8)
         points["decode_1x131072_63x2048_ms_per_step"] = round(dtu * 1e3, 3)
         points["decode_1x131072_63x2048_hbm_frac"] = round(
-            (weight_bytes(cfg, itemsize) + (sum(ctxs) - 64 * 16) * kv_bytes_per_token(cfg, itemsize)) / dtu / HBM_BYTES_PER_S, 4)
+            (weight_bytes(cfg, itemsize, args.weights) + (sum(ctxs) - 64 * 16) * kv_bytes_per_token(cfg, itemsize)) / dtu / HBM_BYTES_PER_S, 4)
         log("decode of 1 x 131,072 + 63 x 2,048 tokens: %.3f ms a step" % (dtu * 1e3))
-    if not (args.no_points or args.no_workloads) and args.shape == "1b" and args.layers == layers_full:
+    if (not (args.no_points or args.no_workloads) and args.shape == "1b" and args.layers == layers_full
+            and args.weights == "stored"):
         # the family's other two shapes with the workloads named for them, each on an engine of its own
         del gen, engine
         import gc
@@ -557,6 +562,8 @@ def main() -> int:
                      "frac_measured": round(achieved / peaks["read_GBs"], 4)},
         "points": points,
     }
+    if args.weights != "stored":
+        out["config"]["weights"] = "layers in MXFP4, embedding and output matrix in " + short
     print(json.dumps(out), flush=True)
     return 0
 

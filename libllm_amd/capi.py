@@ -12,7 +12,7 @@ from typing import Iterator, Optional
 
 from .errors import ConfigError, RequestError
 
-_LOAD_KEYS = {"filename", "device", "dtype", "max_tokens", "max_batch", "random_weights", "seed"}
+_LOAD_KEYS = {"filename", "device", "dtype", "max_tokens", "max_batch", "random_weights", "seed", "weights"}
 _GENERATE_KEYS = {"prompts", "max_new_tokens", "temperature", "top_k", "top_p", "seed", "stop_tokens"}
 _STEP_KEYS = {"step", "entries", "end"}
 _COMPLETE_KEYS = {"messages", "token_ids", "temperature", "top_k", "top_p", "max_new_tokens", "seed", "stop_ids"}
@@ -25,8 +25,8 @@ def parse(text: str) -> str:
 
 def load(kwargs_json: str):
     """``filename``: the model folder or its config.json; ``device``: cpu, cuda or auto
-    (src/libllm/llm.cc:154-168, 206-236).  Ours: ``dtype``, ``max_tokens``, ``max_batch``, and
-    ``random_weights`` with ``seed`` (only config.json is then read)."""
+    (src/libllm/llm.cc:154-168, 206-236).  Ours: ``dtype``, ``max_tokens``, ``max_batch``,
+    ``weights`` ("stored" or "mxfp4"), and ``random_weights`` with ``seed`` (only config.json is then read)."""
     from .api import Model, parse_device
     kw = json.loads(kwargs_json)
     if not isinstance(kw, dict):
@@ -38,7 +38,8 @@ def load(kwargs_json: str):
         raise ConfigError("key \"filename\" is required")
     return Model(kw["filename"], parse_device(str(kw.get("device", "auto"))), dtype=kw.get("dtype", "bfloat16"),
                  max_tokens=int(kw.get("max_tokens", 8192)), max_batch=int(kw.get("max_batch", 64)),
-                 random_weights=bool(kw.get("random_weights", False)), seed=int(kw.get("seed", 0)))
+                 random_weights=bool(kw.get("random_weights", False)), seed=int(kw.get("seed", 0)),
+                 weights=str(kw.get("weights", "stored")))
 
 
 def info(model) -> str:

@@ -40,6 +40,8 @@ def _model_args(prog):
           help="the model folder (config.json and model.safetensors)")
     _flag(ap, "device", default="auto", help="inference device, either cpu, cuda (or hip) or auto")
     _flag(ap, "dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"])
+    _flag(ap, "weights", default="stored", choices=["stored", "mxfp4"],
+          help="the layers' matrices as the file stores them, or in microscaled 4-bit floating point")
     _flag(ap, "random_weights", action="store_true",
           help="read only config.json from the model folder and draw the weights from -seed")
     _flag(ap, "max_tokens", type=int, default=8192, help="tokens the cache holds")
@@ -56,7 +58,7 @@ def _load(args, ap):
         ap.error("only 1 model (-m) is expected")
     from .api import Model
     return Model(args.m[0], device, dtype=args.dtype, max_tokens=args.max_tokens,
-                 random_weights=args.random_weights, seed=getattr(args, "seed", 0))
+                 random_weights=args.random_weights, seed=getattr(args, "seed", 0), weights=args.weights)
 
 
 def chat_main(argv) -> int:

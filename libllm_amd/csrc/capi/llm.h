@@ -41,7 +41,7 @@ int32_t llm_json_parse(llm_json_t *j, const char *json_str);
 int32_t llm_json_dump(llm_json_t *j, char *buf, int64_t buf_size);
 
 /* model: kwargs of load {"filename", "device"} (ours: "dtype", "max_tokens", "max_batch",
- * "random_weights", "seed");
+ * "random_weights", "seed", "weights": "stored" or "mxfp4");
  * info {"name", ...}; kwargs of complete {"messages" or "token_ids", "temperature", "top_k",
  * "top_p"} (ours: "max_new_tokens", "seed") */
 int32_t llm_model_init(llm_model_t *m);

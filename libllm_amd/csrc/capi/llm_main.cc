@@ -3,7 +3,7 @@
 //
 //   llm chat -m MODEL [-device cpu|cuda|hip|auto] [-dtype bfloat16|float32] [-max_tokens N]
 //            [-temperature T] [-top_k K] [-top_p P] [-seed S] [-max_new_tokens N] [-ids]
-//            [-random_weights] [-stop_id ID]...
+//            [-random_weights] [-weights stored|mxfp4] [-stop_id ID]...
 //
 // A prompt loop with `:new` (clear the history), `:sys <prompt>` (set the system prompt and clear),
 // empty lines ignored, end of input leaving; after each reply `(N tokens, time=..s, ..ms per token)`.
@@ -40,7 +40,7 @@ void chat_usage() {
   std::fprintf(stderr,
                "usage: llm chat -m MODEL [-device DEVICE] [-dtype {bfloat16,float32}] [-max_tokens N]\n"
                "                [-temperature T] [-top_k K] [-top_p P] [-seed S] [-max_new_tokens N] [-ids]\n"
-               "                [-random_weights] [-stop_id ID]...\n");
+               "                [-random_weights] [-weights {stored,mxfp4}] [-stop_id ID]...\n");
 }
 
 [[noreturn]] void arg_error(const std::string &msg) {
@@ -149,7 +149,7 @@ std::string lower(std::string s) {
 
 int chat_main(int argc, char **argv) {
   std::vector<std::string> models;
-  std::string device = "auto", dtype = "bfloat16";
+  std::string device = "auto", dtype = "bfloat16", weights = "stored";
   long max_tokens = 8192, top_k = 50, seed = 0, max_new = 256;
   double temperature = 1.0, top_p = 0.8;
   bool ids = false, random_weights = false;
@@ -170,6 +170,7 @@ int chat_main(int argc, char **argv) {
     if (flag == "m") models.push_back(value);
     else if (flag == "device") device = lower(value);
     else if (flag == "dtype") dtype = value;
+    else if (flag == "weights") weights = value;
     else if (flag == "max_tokens") max_tokens = as_long();
     else if (flag == "temperature") temperature = as_double();
     else if (flag == "top_k") top_k = as_long();
@@ -182,6 +183,7 @@ int chat_main(int argc, char **argv) {
   if (device != "cpu" && device != "cuda" && device != "hip" && device != "auto")
     arg_error("invalid device name: must be one of \"cpu\", \"cuda\" or \"auto\"");
   if (dtype != "bfloat16" && dtype != "float32" && dtype != "bf16" && dtype != "fp32") arg_error("argument -dtype: invalid choice: '" + dtype + "'");
+  if (weights != "stored" && weights != "mxfp4") arg_error("argument -weights: invalid choice: '" + weights + "'");
   if (models.empty()) arg_error("model name (-m) is empty.");
   if (models.size() != 1) arg_error("only 1 model (-m) is expected");
 
@@ -197,7 +199,7 @@ int chat_main(int argc, char **argv) {
     std::ostringstream js;
     js << "{\"filename\": " << quoted(models[0]) << ", \"device\": " << quoted(device) << ", \"dtype\": "
        << quoted(dtype) << ", \"max_tokens\": " << max_tokens << ", \"random_weights\": "
-       << (random_weights ? "true" : "false") << ", \"seed\": " << seed << "}";
+       << (random_weights ? "true" : "false") << ", \"seed\": " << seed << ", \"weights\": " << quoted(weights) << "}";
     CHECK(llm_json_parse(&kwargs, js.str().c_str()));
     CHECK(llm_model_load(&model, &kwargs));
   }

@@ -2,7 +2,11 @@
 // W: X in bfloat16 (W's codes are widened to bfloat16, exactly, in front of
 // v_mfma_f32_16x16x32_bf16) or in MXFP4 too (v_mfma_scale_f32_16x16x128_f8f6f4 takes both as they
 // lie).  Sums in float32, result bfloat16 or float32, or gated over a stacked [gate; up] weight
-// (out[m, i] = act(gate_i) * up_i, both still in 32 bits: one rounding).
+// (out[m, i] = act(gate_i) * up_i, both still in 32 bits: one rounding), or added into the residual
+// stream, or rotated and written to the cache.  With rows in bfloat16 an RMS norm between two products
+// needs no kernel of its own up to 16 rows, as in the product for few rows with bfloat16 weights (there
+// is why): the product that adds into the stream prepares it, the product behind it multiplies its sums
+// by the row's scale.
 //
 // The waves of a block split K, a run of units of 128 elements each, and every wave goes through its
 // run alone, with no barrier until the waves' sums are added at the end, in their order.  W goes from
@@ -14,9 +18,12 @@
 // different elements of X, so sharing them would gain nothing.  Which wave adds which unit does not
 // depend on M: an output is the same bits whatever else is in the batch.
 #include "mx4.h"
+#include "row_epilogue.h"
 
 #define MR_EPI_NONE 0
 #define MR_EPI_GATED 1
+#define MR_EPI_ACCUM 2
+#define MR_EPI_ROPE 3
 
 struct Mx4Args {
   const bf16_t* X;           // rows in bfloat16, ldx elements apart (a multiple of 8, K too), or null:
@@ -30,11 +37,17 @@ struct Mx4Args {
   int n_out;                 // columns of C: N, or N / 2 if gated
   int ldx, units, quads, act;   // units: those that hold elements of K
   hipStream_t stream;
+  const float* next_w;       // accumulating: weight [N] of the norm that reads the stream next, or null
+  bf16_t* raw;               //   out [M, N]: the new stream times next_w
+  float* ssq_out;            //   out [M, N / 16]: sums of squares of the new stream over tiles of 16 columns
+  const float* ssq_in;       // [M, K / 16]: such sums for the rows of X, which still lack their scale; or null
+  float eps;
+  RowRope rope;
 };
 
 // WAVES: waves that split K; MT: tiles of 16 rows of X; XQ: quarters of a tile of which rows exist (4 unless MT is 1);
 // RT: tiles of W a wave; STAGES: units in flight.
-template <int WAVES, int MT, int XQ, int RT, int STAGES, int EPI, typename OutT, bool X4>
+template <int WAVES, int MT, int XQ, int RT, int STAGES, int EPI, bool NORM, typename OutT, bool X4>
 __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
   constexpr int RPR = EPI == MR_EPI_GATED ? 2 : 1;        // tiles of W that make one tile of outputs
   constexpr int OUT_RT = RT / RPR;
@@ -44,6 +57,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
   float* red = reinterpret_cast<float*>(lds);
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
+  __shared__ float s_scale[16];                           // a row's rsqrt(mean(x^2) + eps) where X lacks it
   const int out_tile0 = blockIdx.x * OUT_RT, m0 = blockIdx.y * (16 * MT);
   const int out_tiles = (a.n_out + 15) / 16;
   unsigned char* mine = lds + wave * WAVE_B;
@@ -149,21 +163,64 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
   // this wave's run of units
   const int per = (a.units + WAVES - 1) / WAVES;
   const int first = wave * per, last = min(a.units, first + per);
-  if (first < last) {
-    Stage st[STAGES];
+  // What the epilogue needs from memory beside the sums is asked for in front of the first loads: the wave
+  // of a row tile finishes its columns 4 g .. 4 g + 3, 16 apart a round.  No branch here: one between the
+  // first loads and the loop makes the compiler hold everything in flight twice.
+  const int e_m = m0 + wave * 16 + r, e_n0 = out_tile0 * 16 + 4 * g;
+  const int e_row = min(e_m, a.M - 1);                     // (a row that exists; what belongs to another is not stored)
+  RopeSteps<EPI == MR_EPI_ROPE ? OUT_RT : 1> e_rope;
+  float e_prev[EPI == MR_EPI_ACCUM ? OUT_RT : 1][4], e_nw[EPI == MR_EPI_ACCUM && NORM ? OUT_RT : 1][4];
+  if constexpr (EPI == MR_EPI_ROPE) e_rope.first(a.rope, e_row);
+  if constexpr (EPI == MR_EPI_ACCUM) {
 #pragma unroll
-    for (int d = 0; d < STAGES; ++d) load(min(first + d, last - 1), st[d]);
-    int u = first;
-    for (; u + STAGES <= last; u += STAGES) {
+    for (int ort = 0; ort < OUT_RT; ++ort)
 #pragma unroll
-      for (int d = 0; d < STAGES; ++d) {
-        compute(u + d, st[d]);
-        load(min(u + d + STAGES, last - 1), st[d]);      // (past the end: the last unit again, unused)
+      for (int e = 0; e < 4; ++e) {
+        const int n = min(e_n0 + ort * 16 + e, a.n_out - 1);
+        e_prev[ort][e] = ((const float*)a.C)[(size_t)e_row * a.n_out + n];
+        if constexpr (NORM) e_nw[ort][e] = a.next_w[n];
       }
-    }
+  }
+  // The sums of squares of a row of X that still lacks its scale: TPR neighbouring threads a row.
+  constexpr int TPR = WAVES * 4, SS_AHEAD = 8;
+  static_assert(TPR <= 64, "the threads of a row lie in one wave");
+  constexpr bool SCALES = NORM && EPI != MR_EPI_ACCUM;
+  static_assert(!NORM || (MT == 1 && !X4), "norms are folded for up to 16 rows in bfloat16");
+  float e_ss[SS_AHEAD];
+  const int ss_row = tid / TPR, ss_part = tid % TPR, parts_in = a.K / 16;
+  const size_t ss_at = (size_t)min(ss_row, a.M - 1) * parts_in;
+  if constexpr (SCALES) {
 #pragma unroll
-    for (int d = 0; d < STAGES - 1; ++d)
-      if (u + d < last) compute(u + d, st[d]);
+    for (int i = 0; i < SS_AHEAD; ++i) {
+      const int p = ss_part + i * TPR;
+      const float q = a.ssq_in[ss_at + min(p, parts_in - 1)];
+      e_ss[i] = p < parts_in ? q : 0.f;
+    }
+  }
+  Stage st[STAGES];
+#pragma unroll
+  for (int d = 0; d < STAGES; ++d) load(min(first + d, a.units - 1), st[d]);      // (a wave may have none)
+  if constexpr (EPI == MR_EPI_ROPE) e_rope.second(a.rope, e_n0);
+  int u = first;
+  for (; u + STAGES <= last; u += STAGES) {
+#pragma unroll
+    for (int d = 0; d < STAGES; ++d) {
+      compute(u + d, st[d]);
+      load(min(u + d + STAGES, last - 1), st[d]);        // (past the end: the last unit again, unused)
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < STAGES - 1; ++d)
+    if (u + d < last) compute(u + d, st[d]);
+  if constexpr (EPI == MR_EPI_ROPE) e_rope.third(a.rope);
+  if constexpr (SCALES) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < SS_AHEAD; ++i) ss += e_ss[i];
+    for (int p = ss_part + SS_AHEAD * TPR; p < parts_in; p += TPR) ss += a.ssq_in[ss_at + p];      // wider rows
+#pragma unroll
+    for (int off = TPR / 2; off >= 1; off >>= 1) ss += __shfl_xor(ss, off, 64);
+    if (ss_part == 0) s_scale[ss_row] = rsqrtf(ss / (float)a.K + a.eps);      // read behind the next barrier
   }
 
   // ---- the waves' sums, added in order through shared memory (a wave writes where its rows of X
@@ -181,8 +238,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
                         acc[ort * RPR + j][mt][3]);
     __syncthreads();
     if (wave < MT) {
-      const int mt = wave;
-      const int m = m0 + mt * 16 + r, n = (out_tile0 + ort) * 16 + 4 * g;
+      const int mt = wave, m = e_m, n = e_n0 + ort * 16;
       float v[RPR][4];
 #pragma unroll
       for (int j = 0; j < RPR; ++j) {
@@ -193,11 +249,26 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
           s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
         }
         v[j][0] = s.x; v[j][1] = s.y; v[j][2] = s.z; v[j][3] = s.w;
+        if constexpr (SCALES) {
+          const float sc = s_scale[r];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] *= sc;
+        }
       }
-      if (m < a.M && n < a.n_out) {
+      const bool on = m < a.M && n < a.n_out;
+      if constexpr (EPI == MR_EPI_ROPE) {
+        if (on) rope_store<OUT_RT>(a.rope, e_rope, ort, v[0], m, n, (bf16_t*)a.C);
+        continue;
+      }
+      if constexpr (EPI == MR_EPI_ACCUM && NORM) {
+        norm_store(on, v[0], e_prev[ort], e_nw[ort], m, n, a.n_out, g, (float*)a.C, a.raw, a.ssq_out);
+        continue;
+      }
+      if (on) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           if (EPI == MR_EPI_GATED) v[0][e] = llm_gated(a.act, v[0][e], v[RPR - 1][e]);
+          else if (EPI == MR_EPI_ACCUM) v[0][e] += e_prev[ort][e];
           else if (a.bias != nullptr && n + e < a.n_out) v[0][e] += a.bias[n + e];
         }
         OutT* dst = (OutT*)a.C + (size_t)m * a.n_out + n;
@@ -213,13 +284,13 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
   }
 }
 
-template <int WAVES, int MT, int XQ, int RT, int STAGES, int EPI, typename OutT, bool X4>
+template <int WAVES, int MT, int XQ, int RT, int STAGES, int EPI, bool NORM, typename OutT, bool X4>
 static int launch_mx4_rows(const Mx4Args& a) {
   constexpr int OUT_RT = EPI == MR_EPI_GATED ? RT / 2 : RT;
   const int tiles = (a.n_out + 15) / 16;
   const dim3 grid((tiles + OUT_RT - 1) / OUT_RT, (a.M + 16 * MT - 1) / (16 * MT));
   if (grid.y > 65535) return LLM_ERR_ARG;
-  gemm_mx4_rows_kernel<WAVES, MT, XQ, RT, STAGES, EPI, OutT, X4><<<grid, WAVES * 64, 0, a.stream>>>(a);
+  gemm_mx4_rows_kernel<WAVES, MT, XQ, RT, STAGES, EPI, NORM, OutT, X4><<<grid, WAVES * 64, 0, a.stream>>>(a);
   return llm_launch_status();
 }
 
@@ -230,44 +301,59 @@ static int launch_mx4_rows(const Mx4Args& a) {
 // of 4,096 x 14,336 by 8 rows 20.2 / 26.1 / 28.5).  Two tiles of outputs a wave halve what a block
 // reads of X: from 9 rows on, where tiles are many (that gate and up: 23.0 against 24.1 us by 16 rows,
 // but 17.9 against 16.3 by one).
-template <int MT, int XQ, int STAGES, int EPI, typename OutT, bool X4>
+template <int MT, int XQ, int STAGES, int EPI, bool NORM, typename OutT, bool X4>
 static int pick_mx4_tiles(const Mx4Args& a) {
   constexpr int ONE = EPI == MR_EPI_GATED ? 2 : 1;
   const int tiles = (a.n_out + 15) / 16, units = llm_compute_units();
-  if (tiles <= units / 2) return launch_mx4_rows<16, MT, XQ, ONE, 2, EPI, OutT, X4>(a);
-  if (tiles <= units) return launch_mx4_rows<8, MT, XQ, ONE, STAGES, EPI, OutT, X4>(a);
+  if (tiles <= units / 2) return launch_mx4_rows<16, MT, XQ, ONE, MT == 1 ? 2 : 1, EPI, NORM, OutT, X4>(a);
+  if (tiles <= units) return launch_mx4_rows<8, MT, XQ, ONE, STAGES, EPI, NORM, OutT, X4>(a);
   if constexpr (MT == 1 && XQ == 4 && !X4)
-    if (tiles >= 3 * units) return launch_mx4_rows<4, MT, XQ, 2 * ONE, STAGES, EPI, OutT, X4>(a);
-  return launch_mx4_rows<4, MT, XQ, ONE, STAGES, EPI, OutT, X4>(a);
+    if (tiles >= 3 * units) return launch_mx4_rows<4, MT, XQ, 2 * ONE, STAGES, EPI, NORM, OutT, X4>(a);
+  return launch_mx4_rows<4, MT, XQ, ONE, STAGES, EPI, NORM, OutT, X4>(a);
 }
 
-template <int EPI, typename OutT, bool X4>
+template <int EPI, bool NORM, typename OutT, bool X4>
 static int pick_mx4_rows(const Mx4Args& a) {
   if constexpr (!X4) {
-    if (a.M <= 4) return pick_mx4_tiles<1, 1, 4, EPI, OutT, X4>(a);
-    if (a.M <= 8) return pick_mx4_tiles<1, 2, 4, EPI, OutT, X4>(a);
+    if (a.M <= 4) return pick_mx4_tiles<1, 1, 4, EPI, NORM, OutT, X4>(a);
+    if (a.M <= 8) return pick_mx4_tiles<1, 2, 4, EPI, NORM, OutT, X4>(a);
   }
-  if (a.M <= 16) return pick_mx4_tiles<1, 4, 4, EPI, OutT, X4>(a);
-  return pick_mx4_tiles<2, 4, 3, EPI, OutT, X4>(a);
+  if (a.M <= 16) return pick_mx4_tiles<1, 4, 4, EPI, NORM, OutT, X4>(a);
+  if constexpr (!NORM) return pick_mx4_tiles<2, 4, 3, EPI, NORM, OutT, X4>(a);
+  return LLM_ERR_ARG;
 }
 
 template <bool X4>
 static int mx4_rows(const Mx4Args& a, int epilogue, int out_dtype) {
+#define MR_PICK(EPI, T)                                                                              \
+  do {                                                                                               \
+    if constexpr (!X4)                                                                               \
+      if (a.next_w != nullptr || a.ssq_in != nullptr) return pick_mx4_rows<EPI, true, T, X4>(a);     \
+    return pick_mx4_rows<EPI, false, T, X4>(a);                                                      \
+  } while (0)
   if (epilogue == MR_EPI_NONE) {
-    if (out_dtype == LLM_DTYPE_BF16) return pick_mx4_rows<MR_EPI_NONE, bf16_t, X4>(a);
-    if (out_dtype == LLM_DTYPE_F32) return pick_mx4_rows<MR_EPI_NONE, float, X4>(a);
+    if (out_dtype == LLM_DTYPE_BF16) MR_PICK(MR_EPI_NONE, bf16_t);
+    if (out_dtype == LLM_DTYPE_F32) MR_PICK(MR_EPI_NONE, float);
   } else if (epilogue == MR_EPI_GATED && out_dtype == LLM_DTYPE_BF16) {
-    return pick_mx4_rows<MR_EPI_GATED, bf16_t, X4>(a);
+    MR_PICK(MR_EPI_GATED, bf16_t);
+  } else if (epilogue == MR_EPI_ACCUM && out_dtype == LLM_DTYPE_F32) {
+    if constexpr (!X4) MR_PICK(MR_EPI_ACCUM, float);
   }
+#undef MR_PICK
   return LLM_ERR_ARG;
 }
 
 // W [N, K] as mx4.h lays it out.  X: bfloat16 rows ldx apart (K and ldx multiples of 8, 16-byte
 // aligned) with xs null, or codes with their scales in xs.  epilogue 0: C [M, N] of out_dtype, plus
 // bias[n] if not null; 1 | act << 4: C [M, N / 2] in bfloat16, the gate through an activation of
-// common.h, N / 2 a multiple of 16.
+// common.h, N / 2 a multiple of 16; 2 (bfloat16 rows): added into the float32 C [M, N].
+// Around an RMS norm without a kernel of its own (bfloat16 rows, M at most 16; see gemm_skinny.hip):
+// epilogue 2 with next_w (N a multiple of 16): beside adding, raw [M, N] = bfloat16(C * next_w) and
+// ssq_out [M, N / 16] are written; epilogue 0 or 1 with ssq_in [M, K / 16] (K a multiple of 16): the sums
+// are multiplied by rsqrt(sum(ssq_in[m]) / K + eps) first.
 extern "C" int llm_gemm_mx4_rows(const void* X, const void* xs, int ldx, const void* wc, const void* ws,
                                  const float* bias, void* C, int epilogue, int out_dtype, int M, int N, int K,
+                                 const float* next_w, void* raw, float* ssq_out, const float* ssq_in, float eps,
                                  hipStream_t stream) {
   if (M <= 0) return LLM_OK;
   const int act = epilogue >> 4;
@@ -276,7 +362,12 @@ extern "C" int llm_gemm_mx4_rows(const void* X, const void* xs, int ldx, const v
   if (X == nullptr || wc == nullptr || ws == nullptr || C == nullptr) return LLM_ERR_ARG;
   if ((((uintptr_t)X) | ((uintptr_t)wc) | ((uintptr_t)ws) | ((uintptr_t)C) | ((uintptr_t)xs)) & 15) return LLM_ERR_ARG;
   if (xs == nullptr && (ldx < K || (ldx & 7) || (K & 7))) return LLM_ERR_ARG;
-  if (epilogue == MR_EPI_GATED && ((N & 31) || bias != nullptr)) return LLM_ERR_ARG;
+  if (epilogue == MR_EPI_GATED && (N & 31)) return LLM_ERR_ARG;
+  if (epilogue != MR_EPI_NONE && bias != nullptr) return LLM_ERR_ARG;
+  if (next_w != nullptr && (epilogue != MR_EPI_ACCUM || M > 16 || (N & 15) || raw == nullptr || ssq_out == nullptr ||
+                            (((uintptr_t)raw) & 15)))
+    return LLM_ERR_ARG;
+  if (ssq_in != nullptr && (epilogue == MR_EPI_ACCUM || xs != nullptr || M > 16 || (K & 15) || !(eps >= 0.f))) return LLM_ERR_ARG;
   Mx4Args a{};
   a.X = (const bf16_t*)X;
   a.xc = (const uint4*)X;
@@ -294,5 +385,51 @@ extern "C" int llm_gemm_mx4_rows(const void* X, const void* xs, int ldx, const v
   a.quads = mx4_quads(K);
   a.act = act;
   a.stream = stream;
+  a.next_w = next_w;
+  a.raw = (bf16_t*)raw;
+  a.ssq_out = ssq_out;
+  a.ssq_in = ssq_in;
+  a.eps = eps;
   return xs == nullptr ? mx4_rows<false>(a, epilogue, out_dtype) : mx4_rows<true>(a, epilogue, out_dtype);
+}
+
+// The stacked q|k|v projection with the rotary epilogue: rotated q as bfloat16 [M, n_heads * hd] to
+// q_out, k and v to the cache if write_kv.  W has (n_heads + 2 n_kv) * hd rows with write_kv, else n_heads
+// * hd; hd a multiple of 16, rot_dim even.  ssq_in as above.
+extern "C" int llm_gemm_mx4_rows_rope(const void* X, int ldx, const void* wc, const void* ws, const float* bias,
+                                      void* q_out, int M, int K, int n_heads, int n_kv, int hd, const float* cos_t,
+                                      const float* sin_t, int rot_dim, const int* tok_pos, const int* tok_seq,
+                                      const int* seq_slot, const int* table, int table_stride, void* k_pages,
+                                      void* v_pages, int page_size, int write_kv, const float* ssq_in, float eps,
+                                      hipStream_t stream) {
+  if (M <= 0) return LLM_OK;
+  if (ssq_in != nullptr && (M > 16 || (K & 15) || !(eps >= 0.f))) return LLM_ERR_ARG;
+  if (K <= 0 || (K & 7) || ldx < K || (ldx & 7) || n_heads <= 0 || n_kv < 0 || hd <= 0 || (hd & 15) || rot_dim < 0 ||
+      rot_dim > hd || (rot_dim & 1) || page_size != LLM_PAGE)
+    return LLM_ERR_ARG;
+  if (X == nullptr || wc == nullptr || ws == nullptr || q_out == nullptr || tok_pos == nullptr) return LLM_ERR_ARG;
+  if ((((uintptr_t)X) | ((uintptr_t)wc) | ((uintptr_t)ws) | ((uintptr_t)q_out)) & 15) return LLM_ERR_ARG;
+  if (rot_dim > 0 && (cos_t == nullptr || sin_t == nullptr)) return LLM_ERR_ARG;
+  if (write_kv && (!k_pages || !v_pages || !table || !seq_slot || !tok_seq || n_kv <= 0 ||
+                   ((((uintptr_t)k_pages) | ((uintptr_t)v_pages)) & 7)))
+    return LLM_ERR_ARG;
+  Mx4Args a{};
+  a.X = (const bf16_t*)X;
+  a.wc = (const uint4*)wc;
+  a.ws = (const uint32_t*)ws;
+  a.C = q_out;
+  a.M = M;
+  a.N = (n_heads + (write_kv ? 2 * n_kv : 0)) * hd;
+  a.K = K;
+  a.n_out = a.N;
+  a.ldx = ldx;
+  a.units = mx4_units(K);
+  a.quads = mx4_quads(K);
+  a.stream = stream;
+  a.ssq_in = ssq_in;
+  a.eps = eps;
+  a.rope = RowRope{bias, cos_t, sin_t, tok_pos, tok_seq, seq_slot, table, (bf16_t*)k_pages, (bf16_t*)v_pages,
+                   table_stride, n_heads, n_kv, hd, rot_dim, write_kv};
+  if (ssq_in != nullptr) return pick_mx4_rows<MR_EPI_ROPE, true, bf16_t, false>(a);
+  return pick_mx4_rows<MR_EPI_ROPE, false, bf16_t, false>(a);
 }

@@ -30,7 +30,7 @@
 // order, and multiplies its sums by s before its own epilogue.  The statistics are those of the
 // 32-bit stream, as in the norm kernel (src/flint/cuda/rms_norm.cu:45-76); a row is rounded once,
 // before instead of after its scale.
-#include "mfma.h"
+#include "row_epilogue.h"
 
 #define SK_WK 8            // waves that split K
 #define SK_EPI_NONE 0
@@ -42,19 +42,6 @@
 
 // MT: 16-row tiles of X; RT: 16-row tiles of W per wave; WN: row groups per block; G: granules of
 // 2 steps that a wave takes per chunk (a chunk is 512*G elements of K).
-struct SkinnyRope {
-  const float* bias;       // [N] or null
-  const float* cos_t;      // [positions, rot_dim / 2]
-  const float* sin_t;
-  const int* tok_pos;      // [M] position of each row's token
-  const int* tok_seq;      // [M] its sequence in the step
-  const int* seq_slot;     // [sequences] slot of each sequence
-  const int* table;        // [slots, table_stride] page of (slot, position / 64)
-  bf16_t* k_pages;
-  bf16_t* v_pages;
-  int table_stride, n_heads, n_kv, hd, rot_dim, write_kv;
-};
-
 struct SkinnyNorm {
   const float* next_w;     // accumulating epilogue: weight [N] of the norm that reads the stream next, or null
   bf16_t* raw;             //   out [M, N]: the new stream times next_w
@@ -71,7 +58,7 @@ __global__ __launch_bounds__(WN* SK_WK * 64) void gemm_skinny_kernel(const bf16_
                                                                       OutT* __restrict__ C, int M,
                                                                       int N, int K, int ldw,
                                                                       int n_out, int ldx, int w_steps,
-                                                                      SkinnyRope rope, SkinnyNorm norm) {
+                                                                      RowRope rope, SkinnyNorm norm) {
   constexpr int NT = WN * SK_WK * 64;
   constexpr int CK = 512 * G;                    // elements of K per chunk
   constexpr int ROW_B = CK * 2;                  // bytes of a staged row; 16-byte pieces are swizzled
@@ -196,32 +183,10 @@ __global__ __launch_bounds__(WN* SK_WK * 64) void gemm_skinny_kernel(const bf16_
   const int e_m = e_mt * 16 + (e_ln & 15);
   const int e_n0 = (blockIdx.x * WN + e_wn) * OUT_RT * 16 + 4 * (e_ln >> 4);   // round ort adds 16 * ort
   const bool e_on = tid < ITEMS && e_m < M;
-  int e_pos = 0, e_page = 0;
-  float2 e_cos[EPI == SK_EPI_ROPE ? OUT_RT : 1], e_sin[EPI == SK_EPI_ROPE ? OUT_RT : 1];
+  RopeAhead<EPI == SK_EPI_ROPE ? OUT_RT : 1> e_rope;
   float e_prev[EPI == SK_EPI_ACCUM ? OUT_RT : 1][4], e_nw[EPI == SK_EPI_ACCUM ? OUT_RT : 1][4];
-  if (EPI == SK_EPI_ROPE && e_on) {
-    e_pos = rope.tok_pos[e_m];
-    const int q_dim = rope.n_heads * rope.hd, kv_dim = rope.n_kv * rope.hd;
-#pragma unroll
-    for (int ort = 0; ort < OUT_RT; ++ort) {
-      const int n = e_n0 + ort * 16, d = n % rope.hd;
-      e_cos[ort] = make_float2(1.f, 1.f);
-      e_sin[ort] = make_float2(0.f, 0.f);
-      if (n < q_dim + kv_dim && d < rope.rot_dim) {       // rot_dim is even; d is a multiple of 4
-        const float* cr = rope.cos_t + (size_t)e_pos * (rope.rot_dim / 2) + (d >> 1);
-        const float* sr = rope.sin_t + (size_t)e_pos * (rope.rot_dim / 2) + (d >> 1);
-        e_cos[ort].x = cr[0];
-        e_sin[ort].x = sr[0];
-        if (d + 2 < rope.rot_dim) {
-          e_cos[ort].y = cr[1];
-          e_sin[ort].y = sr[1];
-        }
-      }
-    }
-    if (rope.write_kv && e_n0 + (OUT_RT - 1) * 16 >= q_dim) {
-      const int slot = rope.seq_slot[rope.tok_seq[e_m]];
-      e_page = rope.table[(size_t)slot * rope.table_stride + e_pos / 64];
-    }
+  if constexpr (EPI == SK_EPI_ROPE) {
+    if (e_on) e_rope.load(rope, e_m, e_n0);
   }
   if (EPI == SK_EPI_ACCUM && e_on) {
 #pragma unroll
@@ -340,67 +305,15 @@ __global__ __launch_bounds__(WN* SK_WK * 64) void gemm_skinny_kernel(const bf16_
       for (int e = 0; e < 4; ++e) v[e] = (norm.ssq_in != nullptr) ? sum[e] * sc : sum[e];
     }
     const int m = e_m;
-    if (EPI == SK_EPI_ROPE) {
-      if (m >= M || n >= N) continue;                 // N, hd are multiples of 16: four outputs, one head
-      if (rope.bias) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] += rope.bias[n + e];
-      }
-      const int q_dim = rope.n_heads * rope.hd, kv_dim = rope.n_kv * rope.hd;
-      const int pos = e_pos;
-      const int d = n % rope.hd;
-      {                                               // q and k rotate; elsewhere the angle is zero
-        const float c0 = e_cos[ort].x, s0 = e_sin[ort].x, c1 = e_cos[ort].y, s1 = e_sin[ort].y;
-        const float a0 = v[0], a1 = v[1], a2 = v[2], a3 = v[3];
-        v[0] = a0 * c0 - a1 * s0;
-        v[1] = a1 * c0 + a0 * s0;
-        v[2] = a2 * c1 - a3 * s1;
-        v[3] = a3 * c1 + a2 * s1;
-      }
-      uint2 pk;
-      pk.x = pack2_bf16(v[0], v[1]);
-      pk.y = pack2_bf16(v[2], v[3]);
-      if (n < q_dim) {
-        *reinterpret_cast<uint2*>(C + (size_t)m * q_dim + n) = pk;
-      } else if (rope.write_kv) {
-        const int page = e_page;
-        const int kn = n - q_dim;
-        if (kn < kv_dim) {
-          const int kvh = kn / rope.hd;
-          *reinterpret_cast<uint2*>(rope.k_pages + ((size_t)page * rope.n_kv + kvh) * llm_key_block(rope.hd) +
-                                    llm_key_offset(pos % 64, d)) = pk;
-        } else {
-          const int kvh = (kn - kv_dim) / rope.hd;
-          bf16_t* vp = rope.v_pages + ((size_t)page * rope.n_kv + kvh) * llm_value_block(rope.hd) +
-                       llm_value_offset(rope.hd, d, pos % 64);         // dims d .. d + 3 lie 32 apart
-          vp[0] = (bf16_t)(pk.x & 0xffffu);
-          vp[32] = (bf16_t)(pk.x >> 16);
-          vp[64] = (bf16_t)(pk.y & 0xffffu);
-          vp[96] = (bf16_t)(pk.y >> 16);
-        }
-      }
+    if constexpr (EPI == SK_EPI_ROPE) {
+      if (m < M && n < N) rope_store(rope, e_rope, ort, v, m, n, C);   // N, hd are multiples of 16: four outputs, one head
       continue;
     }
-    if (EPI == SK_EPI_ACCUM && norm.next_w != nullptr) {
-      // (N is a multiple of 16 here: a tile is whole or absent; every lane of the wave comes along)
-      const bool on = m < M && n < ldc;
-      float ss = 0.f;
-      if (on) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          v[e] += e_prev[ort][e];
-          ss += v[e] * v[e];
-        }
-        *reinterpret_cast<float4*>(C + (size_t)m * ldc + n) = make_float4(v[0], v[1], v[2], v[3]);
-        uint2 pk;
-        pk.x = pack2_bf16(v[0] * e_nw[ort][0], v[1] * e_nw[ort][1]);
-        pk.y = pack2_bf16(v[2] * e_nw[ort][2], v[3] * e_nw[ort][3]);
-        *reinterpret_cast<uint2*>(norm.raw + (size_t)m * ldc + n) = pk;
+    if constexpr (EPI == SK_EPI_ACCUM) {
+      if (norm.next_w != nullptr) {
+        norm_store(m < M && n < ldc, v, e_prev[ort], e_nw[ort], m, n, ldc, ln >> 4, C, norm.raw, norm.ssq_out);
+        continue;
       }
-      ss += __shfl_xor(ss, 16, 64);                  // the four lanes that hold a row's 16 columns
-      ss += __shfl_xor(ss, 32, 64);
-      if (on && (ln >> 4) == 0) norm.ssq_out[(size_t)m * (ldc / 16) + n / 16] = ss;
-      continue;
     }
     if (m >= M || n >= ldc) continue;
     OutT* dst = C + ((size_t)blockIdx.y * M + m) * ldc + n;
@@ -433,7 +346,7 @@ struct SkinnyArgs {
   int M, N, K, ldw, n_out;     // ldw: elements between rows of W (a multiple of 8, at least K)
   int k_split;                 // slices of K, each to a result matrix of its own (1: the whole product)
   hipStream_t stream;
-  SkinnyRope rope;
+  RowRope rope;
   SkinnyNorm norm;
 };
 
@@ -533,7 +446,7 @@ static int skinny_product(const void* X, const void* W, void* C, int epilogue, i
   a.n_out = N;
   a.k_split = k_split;
   a.stream = stream;
-  a.rope = SkinnyRope{};
+  a.rope = RowRope{};
   a.norm = norm;
   if (epilogue == SK_EPI_NONE) {
     if (out_dtype == LLM_DTYPE_BF16) return pick_shape<SK_EPI_NONE, bf16_t>(a);

@@ -11,7 +11,7 @@ import torch
 
 from ..errors import KernelError
 
-_vp, _i, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t
+_vp, _i, _f, _sz = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_size_t
 
 BLOCK = 32                      # elements that share a scale
 TILE_ROWS, QUAD = 16, 512       # a tile holds 16 rows by whole quads of 512 elements
@@ -21,7 +21,9 @@ SIGNATURES = {
     "llm_mx4_dequantize": [_vp, _vp, _vp, _i, _i, _i, _vp],
     "llm_mx4_pack": [_vp, _sz, _vp, _i, _i, _vp, _vp, _vp],
     "llm_pad_rows": [_vp, _sz, _vp, _i, _i, _i, _vp],
-    "llm_gemm_mx4_rows": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp],
+    "llm_gemm_mx4_rows": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _f, _vp],
+    "llm_gemm_mx4_rows_rope": [_vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _vp, _i, _vp, _vp, _vp, _vp, _i,
+                               _vp, _vp, _i, _i, _vp, _f, _vp],
     "llm_gemm_mx4_many": [_vp, _vp, _i, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _vp],
     "llm_mx4_join": [_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp],
 }
@@ -225,49 +227,87 @@ class Mx4Ops:
         self._launch("llm_pad_rows", at, ld, padded.data_ptr(), x.shape[0], k, ldp)
         return padded, ldp
 
-    def _mx4_product(self, x, w, n_out, out_dtype, epilogue, bias=None):
+    def _mx4_product(self, x, w, n_out, out_dtype, epilogue, bias=None, stack=False):
+        """The product of ``x`` (a matrix, MXFP4 rows, or a record of normed rows whose norm is
+        prepared) with ``w``.  ``stack``: where K goes in slices their products may come back
+        unadded, ``[slices, m, n]`` in 32 bits."""
         self._mx4(w, "the weight")
         n, k = w.shape
-        m, k2 = x.shape
+        pre = getattr(x, "pre", None)
+        m, k2 = pre.raw.shape if pre is not None else x.shape
         if k != k2:
             raise KernelError("linear: x is [%d, %d] but the weight is [%d, %d]" % (m, k2, n, k))
         code = self._dtype_code(out_dtype)
         bptr = None if bias is None else self._dev(bias, "bias", torch.float32, (n,))
-        out = torch.empty((m, n_out), dtype=out_dtype, device=self.device)
         if m == 0:
-            return out
+            return torch.empty((m, n_out), dtype=out_dtype, device=self.device)
         four = isinstance(x, Mx4Matrix)
         form, ks = self._mx4_plan(m, n, n_out, k, four)
         piece = 8 if form < 0 else 128
+        ssq, eps = None, 0.0
         if four:
             self._mx4(x, "linear input")
             xp, xs, ldx = x.codes_ptr, x.scales_ptr, 0
         else:
+            if pre is not None:
+                x, ssq, eps = pre.raw, pre.ssq.data_ptr(), pre.eps
             x, ldx = self._mx4_rows(x, k, piece)
             xp, xs = x.data_ptr(), None
         kp = -(-k // piece) * piece         # (where rows were padded, their length: the weight's codes there are zero)
         wp, ws = w.codes_ptr, w.scales_ptr
-        if form < 0:
-            self._launch("llm_gemm_mx4_rows", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp)
-        elif ks == 1:
-            self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp, form, 1)
-        else:
-            parts = torch.empty((ks, m, n), dtype=torch.float32, device=self.device)
-            self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, None, parts.data_ptr(), self._EPI_NONE,
-                         self._dtype_code(torch.float32), m, n, kp, form, ks)
-            self._launch("llm_mx4_join", parts.data_ptr(), ks, bptr, out.data_ptr(), epilogue, code, m, n)
+        if ks == 1:
+            out = torch.empty((m, n_out), dtype=out_dtype, device=self.device)
+            if form < 0:
+                self._launch("llm_gemm_mx4_rows", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp,
+                             None, None, None, ssq, eps)
+            else:
+                self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp,
+                             form, 1)
+            return out
+        parts = torch.empty((ks, m, n), dtype=torch.float32, device=self.device)
+        self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, None, parts.data_ptr(), self._EPI_NONE,
+                     self._dtype_code(torch.float32), m, n, kp, form, ks)
+        if stack and bias is None and epilogue == self._EPI_NONE:
+            return parts
+        out = torch.empty((m, n_out), dtype=out_dtype, device=self.device)
+        self._launch("llm_mx4_join", parts.data_ptr(), ks, bptr, out.data_ptr(), epilogue, code, m, n)
         return out
 
-    def _linear_mx4(self, x, w, bias, out_dtype, residual=None):
-        """``linear`` with an MXFP4 weight.  With ``residual`` the product is returned, for the norm
-        that comes next to add."""
-        x = self._materialise(x, torch.bfloat16)
-        return self._mx4_product(x, w, w.shape[0], out_dtype, self._EPI_NONE, bias)
+    def _mx4_input(self, x, w):
+        """``x`` for a product with ``w``: a record of normed rows goes in as it is where the product before
+        has prepared its norm and the product for few rows takes it, else the norm kernel runs."""
+        pre = getattr(x, "pre", None)
+        if pre is not None and pre.raw.shape[0] <= self.ACCUM_ROWS and w.shape[1] == pre.raw.shape[1]:
+            return x
+        return self._materialise(x, torch.bfloat16)
+
+    def _linear_mx4(self, x, w, bias, out_dtype, residual=None, then_norm=None):
+        """``linear`` with an MXFP4 weight.  With ``residual`` the product for few rows adds into it;
+        the other returns the product, or its slices of K, for the norm that comes next to add."""
+        x = self._mx4_input(x, w)
+        n, k = w.shape
+        if residual is None or bias is not None or isinstance(x, Mx4Matrix) or getattr(x, "pre", None) is not None:
+            return self._mx4_product(x, w, n, out_dtype, self._EPI_NONE, bias, residual is not None)
+        m = x.shape[0]
+        if m == 0 or x.shape[1] != k or self._mx4_plan(m, n, n, k, False)[0] >= 0:
+            return self._mx4_product(x, w, n, out_dtype, self._EPI_NONE, None, True)
+        self._mx4(w, "the weight")
+        self._dev(residual, "residual stream", torch.float32, (m, n))
+        x, ldx = self._mx4_rows(x, k, 8)
+        record, nw, raw, ssq = None, None, None, None
+        if then_norm is not None and self.fold_norms and m <= self.ACCUM_ROWS and n % 16 == 0:
+            weight, eps = then_norm
+            nw = self._dev(weight, "norm weight", torch.float32, (n,))
+            record = self._prenormed(m, n, weight, eps)
+            raw, ssq = record.raw.data_ptr(), record.ssq.data_ptr()
+        self._launch("llm_gemm_mx4_rows", x.data_ptr(), None, ldx, w.codes_ptr, w.scales_ptr, None, residual.data_ptr(),
+                     self._EPI_ACCUM, self._dtype_code(torch.float32), m, n, -(-k // 8) * 8, nw, raw, ssq, None, 0.0)
+        return record
 
     def _linear_swiglu_mx4(self, x, w, dtype, activation):
         """The gated product with a stacked MXFP4 weight.  Gate and up stay in 32 bits until the
         result is rounded."""
-        x = self._materialise(x, torch.bfloat16)
+        x = self._mx4_input(x, w)
         act = self._act(activation)
         dtype = dtype or torch.bfloat16
         n = w.shape[0]
@@ -276,7 +316,31 @@ class Mx4Ops:
         if dtype == torch.bfloat16 and n // 2 % TILE_ROWS == 0:
             return self._mx4_product(x, w, n // 2, dtype, self._EPI_SWIGLU | (act << 4))
         # up's rows begin inside a tile, or the result is wanted in 32 bits: the product in 32 bits, then the gate
-        if x.shape[0] == 0:
+        y = self._mx4_product(x, w, n, torch.float32, self._EPI_NONE)
+        if y.shape[0] == 0:
             return torch.empty((0, n // 2), dtype=dtype, device=self.device)
-        out = self.silu_mul(self._mx4_product(x, w, n, torch.float32, self._EPI_NONE), activation)
+        out = self.silu_mul(y, activation)
         return out if out.dtype == dtype else out.to(dtype)
+
+    def _qkv_rope_mx4(self, x, w, bias, n_heads, n_kv, hd, cos, sin, rot_dim, ctx, kv, write):
+        """The stacked projection with its rotation and cache write in one kernel, or None where the
+        product for few rows does not take it."""
+        x = self._mx4_input(x, w)
+        pre = getattr(x, "pre", None)
+        rows = pre.raw if pre is not None else x
+        if isinstance(rows, Mx4Matrix):
+            return None, x
+        m, k = rows.shape
+        n = w.shape[0]
+        if m == 0 or k != w.shape[1] or self._mx4_plan(m, n, n, k, False)[0] >= 0:
+            return None, x
+        self._mx4(w, "qkv weight")
+        rows, ldx = self._mx4_rows(rows, k, 8)
+        cptr, sptr, bptr, kptr, vptr, tptr, stride = self._rope_operands("qkv_rope", cos, sin, rot_dim, bias, n, ctx, kv, write,
+                                                                         n_kv, hd, torch.bfloat16)
+        q = torch.empty((m, n_heads * hd), dtype=torch.bfloat16, device=self.device)
+        self._launch("llm_gemm_mx4_rows_rope", rows.data_ptr(), ldx, w.codes_ptr, w.scales_ptr, bptr, q.data_ptr(), m,
+                     -(-k // 8) * 8, n_heads, n_kv, hd, cptr, sptr, rot_dim, ctx.tok_pos.data_ptr(), ctx.tok_seq.data_ptr(),
+                     ctx.seq_slot.data_ptr(), tptr, stride, kptr, vptr, 64, 1 if write else 0,
+                     pre.ssq.data_ptr() if pre is not None else None, pre.eps if pre is not None else 0.0)
+        return q, x

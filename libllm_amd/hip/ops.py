@@ -432,6 +432,12 @@ class HipOps(Mx4Ops):
             pre = None
         return NormedRows(res, weight, float(eps), rows, pre)
 
+    def _prenormed(self, m, n, weight, eps) -> Prenormed:
+        """Room for what a product that adds into a stream [m, n] leaves for the norm."""
+        raw = torch.empty((m, n), dtype=torch.bfloat16, device=self.device)
+        ssq = torch.empty((m, n // 16), dtype=torch.float32, device=self.device)
+        return Prenormed(raw, ssq, weight, float(eps))
+
     def _materialise(self, x, dtype):
         if isinstance(x, NormedRows):
             return self.add_rmsnorm(x.res, None, x.weight, x.eps, dtype, x.rows)
@@ -535,7 +541,7 @@ class HipOps(Mx4Ops):
         ``residual`` next, before anything else touches it: where the product adds into the
         stream at up to ``ACCUM_ROWS`` rows it then returns a ``Prenormed`` for ``normed``."""
         if isinstance(w, Mx4Matrix):
-            return self._linear_mx4(x, w, bias, out_dtype, residual)
+            return self._linear_mx4(x, w, bias, out_dtype, residual, then_norm)
         if isinstance(x, Mx4Matrix):
             raise KernelError("linear: rows in MXFP4 need a weight in MXFP4")
         lazy = isinstance(x, NormedRows)
@@ -579,14 +585,13 @@ class HipOps(Mx4Ops):
                 if then_norm is not None and self.fold_norms and n % 16 == 0 and not lazy:
                     weight, eps = then_norm
                     self._dev(weight, "norm weight", torch.float32, (n,))
-                    raw = torch.empty((m, n), dtype=torch.bfloat16, device=self.device)
-                    ssq = torch.empty((m, n // 16), dtype=torch.float32, device=self.device)
+                    record = self._prenormed(m, n, weight, eps)
                     wptr, ldw = self._streamed(w)
                     self._check(self.lib.llm_gemm_skinny_norm_bf16(
                         x.data_ptr(), wptr, residual.data_ptr(), self._EPI_ACCUM, _code(torch.float32),
-                        m, n, k, ldw, weight.data_ptr(), raw.data_ptr(), ssq.data_ptr(), None, 0, 0.0,
+                        m, n, k, ldw, weight.data_ptr(), record.raw.data_ptr(), record.ssq.data_ptr(), None, 0, 0.0,
                         self._stream()), "gemm_skinny_norm_bf16")
-                    return Prenormed(raw, ssq, weight, float(eps))
+                    return record
                 self._skinny(x, w, residual, self._EPI_ACCUM, 0, m)
                 return None
             if m <= self.SKINNY_ROWS or (out_dtype == torch.float32 and not lazy):
@@ -752,6 +757,14 @@ class HipOps(Mx4Ops):
         fused = (dtype == torch.bfloat16 and (adjacent or rot_dim == 0) and hd % 16 == 0
                  and m <= self.SKINNY_ROWS and m == ctx.n_tokens
                  and (not write or (kv is not None and "k" in kv.planes and kv.planes["k"].dtype == torch.bfloat16)))
+        if isinstance(w, Mx4Matrix):
+            if fused:
+                q, x = self._qkv_rope_mx4(x, w, bias, n_heads, n_kv, hd, cos, sin, rot_dim, ctx, kv, write)
+                if q is not None:
+                    return q
+            qkv = self.linear(x, w, None, dtype)
+            self.rope_kv_write(qkv, bias, n_heads, n_kv, hd, cos, sin, rot_dim, ctx, kv, write, adjacent)
+            return qkv
         pre = x.pre if lazy and fused and self._skinny_ok(x, w, m, k) else None
         if pre is not None:
             x, lazy = pre.raw, False             # rows that lack their norm's scale: see Prenormed
@@ -759,25 +772,8 @@ class HipOps(Mx4Ops):
             x, lazy = self._materialise(x, dtype), False
         if fused and self._skinny_ok(x, w, m, k):
             self._weight(self._plain(w), "qkv weight")
-            cptr = sptr = None
-            if rot_dim:
-                if cos is None or cos.shape[1] != rot_dim // 2 or cos.shape != sin.shape:
-                    raise KernelError("qkv_rope: rotary tables do not match rot_dim %d" % rot_dim)
-                if not ctx.captured and ctx.max_ctx > cos.shape[0]:
-                    raise KernelError("qkv_rope: position %d exceeds the rotary table of %d rows"
-                                      % (ctx.max_ctx - 1, cos.shape[0]))
-                cptr, sptr = self._dev(cos, "cos", torch.float32), self._dev(sin, "sin", torch.float32)
-            bptr = None
-            if bias is not None:
-                bptr = self._dev(bias, "qkv bias", torch.float32)
-                if bias.shape[0] < n:
-                    raise KernelError("qkv_rope: the bias is shorter than a row")
-            kptr = vptr = tptr = None
-            stride = 0
-            if write:
-                k_pages, v_pages = self._kv_planes(kv, n_kv, hd, torch.bfloat16)
-                kptr, vptr, tptr = k_pages.data_ptr(), v_pages.data_ptr(), kv.block_table.data_ptr()
-                stride = kv.block_table.shape[1]
+            cptr, sptr, bptr, kptr, vptr, tptr, stride = self._rope_operands(
+                "qkv_rope", cos, sin, rot_dim, bias, n, ctx, kv, write, n_kv, hd, torch.bfloat16)
             xp = self._dev(x, "qkv input", torch.bfloat16)
             q = torch.empty((m, n_heads * hd), dtype=torch.bfloat16, device=self.device)
             wptr, ldw = self._streamed(w)
@@ -792,6 +788,30 @@ class HipOps(Mx4Ops):
         self.rope_kv_write(qkv, bias, n_heads, n_kv, hd, cos, sin, rot_dim, ctx, kv, write, adjacent)
         return qkv
 
+    def _rope_operands(self, what, cos, sin, rot_dim, bias, width, ctx, kv, write, n_kv, hd, dtype):
+        """Checks what a rotation and cache write read beside the rows; returns the pointers (cos, sin, bias,
+        key pages, value pages, page table) and the page table's row stride."""
+        cptr = sptr = None
+        if rot_dim:
+            if cos is None or cos.shape[1] != rot_dim // 2 or cos.shape != sin.shape:
+                raise KernelError("%s: rotary tables do not match rot_dim %d" % (what, rot_dim))
+            if not ctx.captured and ctx.max_ctx > cos.shape[0]:
+                raise KernelError("%s: position %d exceeds the rotary table of %d rows"
+                                  % (what, ctx.max_ctx - 1, cos.shape[0]))
+            cptr, sptr = self._dev(cos, "cos", torch.float32), self._dev(sin, "sin", torch.float32)
+        bptr = None
+        if bias is not None:
+            bptr = self._dev(bias, "qkv bias", torch.float32)
+            if bias.shape[0] < width:
+                raise KernelError("%s: the bias is shorter than a row" % what)
+        kptr = vptr = tptr = None
+        stride = 0
+        if write:
+            k_pages, v_pages = self._kv_planes(kv, n_kv, hd, dtype)
+            kptr, vptr, tptr = k_pages.data_ptr(), v_pages.data_ptr(), kv.block_table.data_ptr()
+            stride = kv.block_table.shape[1]
+        return cptr, sptr, bptr, kptr, vptr, tptr, stride
+
     def rope_kv_write(self, qkv, bias, n_heads, n_kv, hd, cos, sin, rot_dim, ctx, kv, write,
                       adjacent=False):
         m, width = qkv.shape
@@ -801,25 +821,8 @@ class HipOps(Mx4Ops):
         self._dev(qkv, "qkv")
         if m != ctx.n_tokens:
             raise KernelError("rope_kv_write: %d rows for a step of %d tokens" % (m, ctx.n_tokens))
-        cptr = sptr = None
-        if rot_dim:
-            if cos is None or cos.shape[1] != rot_dim // 2 or cos.shape != sin.shape:
-                raise KernelError("rope_kv_write: rotary tables do not match rot_dim %d" % rot_dim)
-            if not ctx.captured and ctx.max_ctx > cos.shape[0]:
-                raise KernelError("rope_kv_write: position %d exceeds the rotary table of %d rows"
-                                  % (ctx.max_ctx - 1, cos.shape[0]))
-            cptr, sptr = self._dev(cos, "cos", torch.float32), self._dev(sin, "sin", torch.float32)
-        bptr = None
-        if bias is not None:
-            bptr = self._dev(bias, "qkv bias", torch.float32)
-            if bias.shape[0] < need:
-                raise KernelError("rope_kv_write: the bias is shorter than a row")
-        kptr = vptr = tptr = None
-        stride = 0
-        if write:
-            k_pages, v_pages = self._kv_planes(kv, n_kv, hd, qkv.dtype)
-            kptr, vptr, tptr = k_pages.data_ptr(), v_pages.data_ptr(), kv.block_table.data_ptr()
-            stride = kv.block_table.shape[1]
+        cptr, sptr, bptr, kptr, vptr, tptr, stride = self._rope_operands(
+            "rope_kv_write", cos, sin, rot_dim, bias, need, ctx, kv, write, n_kv, hd, qkv.dtype)
         self._check(self.lib.llm_rope_kv_write(
             qkv.data_ptr(), _code(qkv.dtype), width, bptr, n_heads, n_kv, hd, cptr, sptr, rot_dim,
             ctx.tok_pos.data_ptr(), ctx.tok_seq.data_ptr(), ctx.seq_slot.data_ptr(), tptr, stride,

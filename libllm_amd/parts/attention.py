@@ -56,9 +56,9 @@ class Attention(Mixer):
         if self.position.rot_dim > spec.head_dim:
             raise ConfigError("rotary dimension %d exceeds head_dim %d"
                               % (self.position.rot_dim, spec.head_dim))
-        self.qkv = Linear(spec.width, self.q_dim + 2 * self.kv_dim)
-        self.q_only = Linear(spec.width, self.q_dim)
-        self.out = Linear(self.q_dim, spec.width)
+        self.qkv = Linear(spec.width, self.q_dim + 2 * self.kv_dim, low_bit=True)
+        self.q_only = Linear(spec.width, self.q_dim, low_bit=True)
+        self.out = Linear(self.q_dim, spec.width, low_bit=True)
         self.cos = self.sin = None
         self.bias = None
         self.adjacent = False
@@ -108,7 +108,7 @@ class Attention(Mixer):
                 if bias is not None:
                     bias = bias[order].contiguous()
         self.qkv.bind(w, ops=ops)
-        self.q_only.bind(self.qkv.weight[:self.q_dim], ops=ops, like=self.qkv.prepared)    # the same storage
+        self.q_only.bind(w[:self.q_dim], ops=ops, like=self.qkv.prepared)    # the same storage
         self.bias = bias                                 # added inside the rotation kernel
         self.out.bind(tensors[s.o_name + ".weight"], ops=ops)
         self.cos, self.sin = self.position.tables(w.device)

@@ -5,7 +5,11 @@ import torch
 
 
 class Linear:
-    def __init__(self, in_features: int, out_features: int):
+    """``low_bit``: the weight may be held in fewer bits where the operations are told to
+    (``ops.weight_format``); an output layer's is not, whose errors nothing averages out."""
+
+    def __init__(self, in_features: int, out_features: int, low_bit: bool = False):
+        self.low_bit = low_bit
         self.in_features = in_features
         self.out_features = out_features
         self.weight: Optional[torch.Tensor] = None
@@ -15,8 +19,14 @@ class Linear:
     def bind(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, ops=None, like=None):
         """``weight`` is the matrix; ``prepared`` is what the products are given: the matrix, or
         what ``ops.prepare_weight`` makes of it (with ``like``, the prepared form of a matrix of
-        which this one is the leading rows)."""
+        which this one is the leading rows).  With a weight in MXFP4 the matrix itself is not
+        kept (``weight`` is None)."""
         assert tuple(weight.shape) == (self.out_features, self.in_features)
+        if self.low_bit and getattr(ops, "weight_format", None) == "mxfp4":
+            self.weight, self.bias = None, bias
+            whole = like is not None and self.out_features % 16 == 0
+            self.prepared = like.leading_rows(self.out_features) if whole else ops.quantize_mx4(weight)
+            return
         self.weight = weight if weight.stride(-1) == 1 else weight.contiguous()
         self.bias = bias
         self.prepared = self.weight

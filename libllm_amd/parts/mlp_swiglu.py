@@ -39,8 +39,8 @@ class SwiGLU(FeedForward):
         if spec.width <= 0 or spec.intermediate <= 0:
             raise ConfigError("feed-forward sizes must be positive")
         self.spec = spec
-        self.gate_up = Linear(spec.width, 2 * spec.intermediate)
-        self.down = Linear(spec.intermediate, spec.width)
+        self.gate_up = Linear(spec.width, 2 * spec.intermediate, low_bit=True)
+        self.down = Linear(spec.intermediate, spec.width, low_bit=True)
 
     def weights(self):
         s = self.spec

@@ -30,14 +30,36 @@ def default_ops():
     return HipOps()
 
 
+WEIGHT_FORMATS = ("stored", "mxfp4")
+
+
+def _bind(model, tensors, ops, dtype, weights):
+    """Binds the tensors, the layers' matrices in the format asked for."""
+    if weights not in WEIGHT_FORMATS:
+        raise ConfigError("weights are %s, not %r" % (" or ".join(WEIGHT_FORMATS), weights))
+    if weights == "mxfp4":
+        if dtype != torch.bfloat16:
+            raise ConfigError("weights in MXFP4 need bfloat16 activations")
+        if not hasattr(ops, "quantize_mx4"):
+            raise ConfigError("these operations know no weights in MXFP4")
+    before = getattr(ops, "weight_format", None)
+    ops.weight_format = weights
+    try:
+        model.bind(tensors, ops, dtype)
+    finally:
+        ops.weight_format = before
+
+
 def load_engine(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, ops=None,
                 max_slots: Optional[int] = None, use_graphs: bool = True,
-                keep_float32: bool = False, tiled_weights: bool = True) -> Engine:
+                keep_float32: bool = False, tiled_weights: bool = True, weights: str = "stored") -> Engine:
     """Reads config.json, chooses the architecture by its ``model_type``, loads the tensors by
     name and returns an engine whose cache holds ``max_tokens`` tokens.  ``keep_float32``: in
     bfloat16 mode a matrix that the file stores in 32-bit stays float32 (true 32-bit products
     for it) instead of becoming bfloat16.  ``tiled_weights=False``: no second, tiled copy of the
-    bfloat16 matrices (half the weight memory; decoding is 5 to 11 % slower)."""
+    bfloat16 matrices (half the weight memory; decoding is 5 to 11 % slower).  ``weights="mxfp4"``:
+    the matrices of attention and feed-forwards are rounded to MXFP4 when they are bound (4.25 bits
+    an element, held once; the embedding and the output matrix stay as they are)."""
     config = config_from_dir(model_dir)
     tdtype = parse_dtype(dtype)
     spec = config.to_spec()
@@ -47,7 +69,7 @@ def load_engine(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, ops=No
         ops.pack_weights = False
     tensors = load_tensors(model_dir, model.declared(), spec.optional_tensors, tdtype, ops.device,
                            keep_float32)
-    model.bind(tensors, ops, tdtype)
+    _bind(model, tensors, ops, tdtype, weights)
     engine = Engine(model, ops, tdtype, max_tokens, max_slots=max_slots, use_graphs=use_graphs)
     engine.config = config
     return engine
@@ -55,11 +77,12 @@ def load_engine(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, ops=No
 
 def random_engine(config, seed: int = 0, dtype="bfloat16", max_tokens: int = 8192, ops=None,
                   max_slots: Optional[int] = None, use_graphs: bool = True, std: float = 0.02,
-                  stored: torch.dtype = torch.bfloat16, tiled_weights: bool = True) -> Engine:
+                  stored: torch.dtype = torch.bfloat16, tiled_weights: bool = True,
+                  weights: str = "stored") -> Engine:
     """The random-weights mode without a file: every tensor the model declares is drawn on the
     device from ``seed`` (matrices normal with ``std``, norm scales 1) and bound as a loaded file
     would be that stores ``stored`` (float32: full significands for the 32-bit path).  ``config``
-    is a typed configuration."""
+    is a typed configuration; ``weights`` as for ``load_engine``."""
     tdtype = parse_dtype(dtype)
     spec = config.to_spec()
     model = DecoderModel(spec)
@@ -72,7 +95,7 @@ def random_engine(config, seed: int = 0, dtype="bfloat16", max_tokens: int = 819
         t = random_tensors({name: declared[name]}, seed, std=std, dtype=stored,
                            device=ops.device)[name]
         tensors[name] = place(t, declared[name], tdtype, ops.device)
-    model.bind(tensors, ops, tdtype)
+    _bind(model, tensors, ops, tdtype, weights)
     engine = Engine(model, ops, tdtype, max_tokens, max_slots=max_slots, use_graphs=use_graphs)
     engine.config = config
     return engine

@@ -400,3 +400,214 @@ def test_on_another_stream(ops):
         got = ops.linear(x, ops.quantize_mx4(w), None, torch.float32)
     side.synchronize()
     assert torch.equal(got, want)
+
+
+# ------------------------------------------------------------------------------- as a layer uses them
+def held(n, k, seed):
+    codes, scales, w = weight(n, k, seed)
+    packed, s = file_form(codes, scales)
+    return packed, s, w
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 64, 96), (3, 77, 200), (16, 2048, 520), (20, 48, 1000), (32, 100, 64),
+                                   (50, 4112, 136), (70, 64, 2100), (140, 96, 5000)])
+def test_added_into_the_stream(ops, m, n, k):
+    """With ``residual`` the product for few rows adds into it; otherwise what comes back is the
+    product, or its slices of K, and the norm kernel adds them."""
+    packed, s, w = held(n, k, n + m)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    x, res = normal((m, k), m, dtype=torch.bfloat16), normal((m, n), n, 3.0)
+    stream = res.cuda()
+    got = ops.linear(x.cuda(), q, None, torch.bfloat16, residual=stream)
+    xd, rd = x.double().numpy(), res.double().numpy()
+    lim = bound(xd, w, k, torch.float32)
+    if got is None:
+        assert m <= 2 * ops.MX4_ROWS
+        total = stream.double().cpu().numpy()
+    else:
+        assert torch.equal(stream.cpu(), res)
+        if got.dim() == 2:
+            lim = bound(xd, w, k, torch.bfloat16)
+        total = rd + got.double().cpu().numpy().reshape(-1, m, n).sum(0)
+    # one more addition in 32 bits, and one for every slice beside the first (less than ten)
+    lim = lim + 10 * HALF_F32 * (np.abs(rd) + np.abs(xd) @ np.abs(w).T)
+    assert (np.abs(total - (rd + xd @ w.T)) <= lim).all()
+
+
+@pytest.mark.parametrize("m", [1, 2, 7, 8, 16])
+@pytest.mark.parametrize("n,k,inter", [(64, 96, 32), (512, 200, 80), (2064, 520, 48), (4096, 64, 1040)])
+def test_norm_between_two_products(ops, m, n, k, inter):
+    """The product that adds into the stream prepares the norm that reads it; the products behind it
+    (plain, gated, with the rotation) take its rows and scale their sums."""
+    pd, sd, wd = held(n, k, 1)
+    pu, su, wu = held(2 * inter, n, 2)
+    down, up = ops.mx4_from_codes(pd.cuda(), sd.cuda(), k), ops.mx4_from_codes(pu.cuda(), su.cuda(), n)
+    x, res = normal((m, k), m, dtype=torch.bfloat16), normal((m, n), 5, 2.0)
+    nw = (1 + 0.2 * normal((n,), 6)).cuda()
+    stream = res.cuda()
+    record = ops.linear(x.cuda(), down, None, torch.bfloat16, residual=stream, then_norm=(nw, 1e-5))
+    plain_stream = res.cuda()
+    assert ops.linear(x.cuda(), down, None, torch.bfloat16, residual=plain_stream) is None
+    assert torch.equal(stream, plain_stream)
+    # the rows: the stream times the weight, rounded once; the sums of squares of 16 columns
+    assert torch.equal(record.raw, (stream * nw).to(torch.bfloat16))
+    sq = (stream.double() ** 2).view(m, n // 16, 16).sum(-1)
+    assert torch.allclose(record.ssq.double(), sq, rtol=2.0 ** -19, atol=0)          # 16 squares and their sum: 2^-24 each
+    lazy = ops.normed(stream, nw, 1e-5, pre=record)
+    s64 = stream.double().cpu().numpy()
+    scale = 1 / np.sqrt((s64 ** 2).mean(1, keepdims=True) + 1e-5)
+    raw = record.raw.double().cpu().numpy()
+    y = ops.linear(lazy, up, None, torch.float32).double().cpu().numpy()
+    # the sums' error, scaled; the scale itself: n / 16 + 4 additions of positive numbers and rsqrt (1 ulp)
+    rel = (n / 16 + 12) * HALF_F32
+    lim = (bound(raw, wu, n, torch.float32) + rel * (np.abs(raw) @ np.abs(wu).T)) * scale * (1 + rel) * 2
+    assert (np.abs(y - (raw @ wu.T) * scale) <= lim).all()
+    sw = ops.linear_swiglu(lazy, up, torch.bfloat16).double().cpu().numpy()
+    g, u = ((raw @ wu.T) * scale)[:, :inter], ((raw @ wu.T) * scale)[:, inter:]
+    dg, du = lim[:, :inter], lim[:, inter:]
+    want = gate("silu", g, u)
+    ls = 1.2 * dg * (np.abs(u) + du) + (np.abs(g) + dg) * du + 2.0 ** -16 * np.abs(g) * np.abs(u)
+    assert (np.abs(sw - want) <= ls + HALF_BF16 * (np.abs(want) + ls) + 1e-38).all()
+    # more rows than the norm is folded for, or another norm, go through the norm kernel
+    other = ops.linear(ops.normed(stream, nw, 1e-6, pre=record), up, None, torch.float32)
+    ref = ops.add_rmsnorm(stream.clone(), None, nw, 1e-6, torch.bfloat16)
+    assert torch.equal(other, ops.linear(ref, up, None, torch.float32))
+
+
+@pytest.mark.parametrize("rot_half", [True, False])
+@pytest.mark.parametrize("write", [True, False])
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("n_heads,n_kv,hd,k,seqs", [
+    (4, 2, 16, 96, [(0, 0, 1)]),
+    (6, 3, 48, 200, [(2, 5, 1), (0, 63, 1), (1, 64, 1)]),
+    (8, 2, 64, 512, [(0, 60, 9), (3, 0, 1), (1, 100, 5)]),
+    (32, 8, 64, 136, [(i, 7 * i, 1) for i in range(17)]),
+    (4, 4, 128, 96, [(0, 3, 30)]),
+    (6, 2, 32, 64, [(0, 0, 90)]),
+])
+def test_stacked_projection(ops, n_heads, n_kv, hd, k, seqs, bias, write, rot_half):
+    """q rotated, k and v in the cache, against float64; from few rows in one kernel, from many by the
+    product and the rotation kernel."""
+    from helpers import make_ctx, make_kv, read_kv
+    n = (n_heads + (2 * n_kv if write else 0)) * hd
+    rot = hd if rot_half else hd // 2
+    m = sum(c for _, _, c in seqs)
+    packed, s, w = held(n, k, 3)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    x = normal((m, k), 4, dtype=torch.bfloat16)
+    b = normal((n,), 5) if bias else None
+    ctx = make_ctx(ops, torch.bfloat16, seqs)
+    slots = 1 + max(c for c, _, _ in seqs)
+    kv = make_kv("cuda", torch.bfloat16, slots, 3, n_kv, hd, seed=2)
+    cos, sin = torch.cos(normal((192, rot // 2), 8)), torch.sin(normal((192, rot // 2), 8))
+    out = ops.qkv_rope(x.cuda(), q, None if b is None else b.cuda(), n_heads, n_kv, hd, cos.cuda(), sin.cuda(), rot, ctx,
+                       kv, write, True, torch.bfloat16)
+    xd = x.double().numpy()
+    y = xd @ w.T + (0 if b is None else b.double().numpy())
+    pos = ctx.tok_pos.cpu().numpy()
+    heads = y.reshape(m, -1, hd).copy()
+    c, sn = cos.double().numpy()[pos][:, None, :], sin.double().numpy()[pos][:, None, :]
+    turned = heads[:, :n_heads + (n_kv if write else 0)]
+    a0, a1 = turned[:, :, 0:rot:2].copy(), turned[:, :, 1:rot:2].copy()
+    turned[:, :, 0:rot:2], turned[:, :, 1:rot:2] = a0 * c - a1 * sn, a1 * c + a0 * sn
+    # a sum in 32 bits, a bias, two products and a sum more, each within 2^-24 of values up to |a0| + |a1|;
+    # rounded to bfloat16 after the rotation, and from many rows also before it and before the bias,
+    # where the value is the product p = y - b and not y
+    base = (bound(xd, w, k, torch.float32) + HALF_F32 * np.abs(y)).reshape(m, -1, hd)
+    pair = lambda t: np.repeat(t.reshape(m, -1, hd // 2, 2).sum(-1), 2, axis=-1)
+    fused = ops._mx4_plan(m, n, n, k, False)[0] < 0
+    if not fused:
+        base = base + HALF_BF16 * (np.abs(xd @ w.T).reshape(m, -1, hd) + base)
+    size = pair(np.abs(y).reshape(m, -1, hd))
+    lim = pair(base) + 4 * HALF_F32 * size + HALF_BF16 * (size + pair(base)) + 1e-38
+    got = out[:, :n_heads * hd].double().cpu().numpy().reshape(m, n_heads, hd)
+    assert (np.abs(got - heads[:, :n_heads]) <= lim[:, :n_heads]).all()
+    if write:
+        row = 0
+        for slot, pos0, count in seqs:
+            keys, values = read_kv(kv, slot, pos0 + count)
+            kd, vd = keys[pos0:].double().numpy(), values[pos0:].double().numpy()
+            rows = slice(row, row + count)
+            assert (np.abs(kd - heads[rows, n_heads:n_heads + n_kv]) <= lim[rows, n_heads:n_heads + n_kv]).all()
+            assert (np.abs(vd - heads[rows, n_heads + n_kv:]) <= lim[rows, n_heads + n_kv:]).all()
+            assert not keys[:pos0].any() and not values[:pos0].any()
+            row += count
+    else:
+        assert not kv.plane("k").any() and not kv.plane("v").any()
+
+
+# ------------------------------------------------------------------------------- whole models
+LAYER_MATRICES = ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")
+
+
+@pytest.fixture(scope="module")
+def models(tmp_path_factory):
+    """Tiny models and, for the plain implementation, their weights with the layers' matrices rounded to
+    MXFP4 by the quantiser above."""
+    from plain import files, llama
+    from tiny import TINY_A, TINY_B, TINY_C, make_model
+    base, out = tmp_path_factory.mktemp("mx4"), {}
+    for name, cfg in (("A", TINY_A), ("B", TINY_B), ("C", TINY_C)):
+        path = make_model(base, cfg, seed=23 + len(name), name=name)
+        cfg_json, weights = files.read_model_dir(path)
+        rounded = {key: values(*quantise(t)) if key.split(".")[-2] in LAYER_MATRICES and t.ndim == 2 else t
+                   for key, t in weights.items()}
+        out[name] = (path, llama.PlainConfig(cfg_json), rounded)
+    return out
+
+
+@pytest.mark.parametrize("use_graphs", [True, False])
+@pytest.mark.parametrize("name", ["A", "B", "C"])
+def test_model_agrees_with_plain(models, tmp_path, name, use_graphs):
+    """Whole prompts, tokens one by one, and batches of unequal requests, with the layers' matrices in
+    MXFP4, against the plain implementation with the same numbers as weights."""
+    import io
+
+    import traces
+    from helpers import assert_logits_close
+    from libllm_amd.engine.trace import replay
+    from libllm_amd.runtime import load_engine
+    from plain import llama
+    path, cfg, weights = models[name]
+    rng = np.random.default_rng(4)
+    lengths = [70, 33, 100, 5, 64, 1]
+    requests = {"r%d" % i: rng.integers(0, cfg.vocab, size=min(n, cfg.max_pos)).tolist() for i, n in enumerate(lengths)}
+    ids = list(requests)
+    groups = [{r: requests[r] for r in ids[0:3]}, {r: requests[r] for r in ids[3:6]}]
+    decode = {"r0": 20, "r1": 32, "r2": 3, "r3": 4, "r4": 1, "r5": 0}
+    exact = {r: llama.logits_all(cfg, weights, t, store=llama.exact) for r, t in requests.items()}
+    stored = {r: llama.logits_all(cfg, weights, t, store=llama.to_bfloat16) for r, t in requests.items()}
+    for mode, steps in (("whole", traces.whole(requests)), ("tail", traces.tail_one_by_one(requests)),
+                        ("batches", traces.batches(groups, decode))):
+        engine = load_engine(path, dtype="bfloat16", max_tokens=traces.max_tokens_needed(steps), use_graphs=use_graphs,
+                             weights="mxfp4")
+        assert engine.model.blocks[0].feed_forward.down.weight is None
+        replay(engine, traces.lines(steps), str(tmp_path / mode), log=io.StringIO())
+        got = traces.collect(steps, str(tmp_path / mode), cfg.vocab)
+        for r, toks in requests.items():
+            out = np.stack([got[r][p] for p in range(len(toks))])
+            assert_logits_close(out, exact[r], "bfloat16", "%s %s %s" % (name, mode, r), stored[r])
+
+
+def test_generation_and_the_other_entry_points(models, tmp_path):
+    """The same greedy tokens from the Python entry point, the C API's loader and random weights bound
+    as MXFP4; refusals."""
+    import json
+
+    from libllm_amd import Model, capi
+    from libllm_amd.errors import ConfigError
+    path = models["B"][0]
+    prompts = [[5, 8, 13, 21], [1, 2, 3, 4, 5, 6, 7, 8, 9], [42]]
+    model = Model(path, max_tokens=1024, weights="mxfp4")
+    want = model.generate(prompts, max_new_tokens=12, temperature=0.0, stop_tokens=())
+    assert all(len(t) == 12 for t in want)
+    other = capi.load(json.dumps({"filename": path, "max_tokens": 1024, "weights": "mxfp4"}))
+    assert other.generate(prompts, max_new_tokens=12, temperature=0.0, stop_tokens=()) == want
+    stored = Model(path, max_tokens=1024)
+    assert stored.engine.model.blocks[0].feed_forward.down.weight is not None       # the format is not kept
+    rnd = Model(path, max_tokens=256, random_weights=True, seed=3, weights="mxfp4")
+    assert len(rnd.generate([[7, 9]], max_new_tokens=4, temperature=0.0, stop_tokens=())[0]) == 4
+    with pytest.raises(ConfigError):
+        Model(path, dtype="float32", weights="mxfp4")
+    with pytest.raises(ConfigError):
+        Model(path, weights="int4")

@@ -1,0 +1,74 @@
+"""MXFP4 matrices on the host: sizes, checks and launch plans.  (What runs on the device:
+test_gpu_mx4.py.)"""
+import random
+
+import pytest
+import torch
+
+from libllm_amd.errors import ConfigError, KernelError
+from libllm_amd.hip.mx4 import Mx4Matrix, Mx4Ops, tiled_sizes
+
+
+def test_tiled_sizes():
+    assert tiled_sizes(1, 1) == (4096, 256)
+    assert tiled_sizes(16, 512) == (4096, 256)
+    assert tiled_sizes(17, 513) == (4 * 4096, 4 * 256)
+    assert tiled_sizes(28672, 4096) == (28672 * 4096 // 2, 28672 * 4096 // 32)
+
+
+def test_matrix_checks_its_storage():
+    codes, scales = torch.zeros(8192, dtype=torch.uint8), torch.zeros(512, dtype=torch.uint8)
+    q = Mx4Matrix((20, 100), codes, scales)
+    assert q.shape == (20, 100) and q.codes is codes and q.scales is scales
+    top = q.leading_rows(16)
+    assert top.shape == (16, 100) and top.codes.shape == (4096,) and top.codes.data_ptr() == codes.data_ptr()
+    for rows in (0, 8, 17, 32):
+        with pytest.raises(KernelError):
+            q.leading_rows(rows)
+    for bad in (((20, 513), codes, scales), ((33, 100), codes, scales), ((20, 100), codes.int(), scales),
+                ((20, 100), codes, scales[:256]), ((20, 100), codes.view(2, 4096), scales),
+                ((20, 100), torch.zeros(8193, dtype=torch.uint8)[1:], scales)):
+        with pytest.raises(KernelError):
+            Mx4Matrix(*bad)
+    room = Mx4Matrix._new(20, 100, "cpu")
+    assert room.codes.shape == (8192,) and room.scales.shape == (512,)
+    assert room.codes_ptr == room.codes.data_ptr() and room.scales_ptr == room.scales.data_ptr()
+
+
+class Host(Mx4Ops):
+    def __init__(self, units=256):
+        self.units, self._mx4_plans = units, {}
+
+
+def test_plans_are_launches_the_kernels_take():
+    """Every slice of K has quads of its own, a form exists, and the number of plans kept is bounded."""
+    ops, rng = Host(), random.Random(1)
+    ops.MX4_PLANS = 50
+    for _ in range(3000):
+        m, n, k = (int(2 ** rng.uniform(0, top)) for top in (14, 17, 16))
+        four = rng.random() < 0.5
+        gated = n % 2 == 0 and rng.random() < 0.5
+        form, ks = ops._mx4_plan(m, n, n // 2 if gated else n, k, four)
+        assert len(ops._mx4_plans) <= 50
+        assert (form, ks) == ops._mx4_plan(m, n, n // 2 if gated else n, k, four)
+        if form < 0:
+            assert ks == 1 and m <= 2 * ops.MX4_ROWS
+            continue
+        assert form in ((0, 1, 2, 3) if four else (0, 2, 3))
+        quads = -(-k // 512)
+        per = -(-quads // ks)
+        assert -(-quads // per) == ks                    # no slice is empty
+
+
+def test_engine_refuses_formats_it_cannot_hold(tmp_path):
+    from libllm_amd.config import config_from_dict
+    from libllm_amd.runtime import random_engine
+    from tiny import TINY_A
+
+    class Ops:
+        device = torch.device("cpu")
+        supports_graphs = False
+    cfg = config_from_dict(TINY_A)
+    for kw in ({"weights": "fp4"}, {"weights": "mxfp4", "dtype": "float32"}, {"weights": "mxfp4"}):
+        with pytest.raises(ConfigError):
+            random_engine(cfg, ops=Ops(), max_tokens=64, **kw)
