@@ -319,7 +319,12 @@ static int pick_mx4_rows(const Mx4Args& a) {
     if (a.M <= 8) return pick_mx4_tiles<1, 2, 4, EPI, NORM, OutT, X4>(a);
   }
   if (a.M <= 16) return pick_mx4_tiles<1, 4, 4, EPI, NORM, OutT, X4>(a);
-  if constexpr (!NORM) return pick_mx4_tiles<2, 4, 3, EPI, NORM, OutT, X4>(a);
+  if constexpr (!NORM) {
+    // 17 to 32 rows of a weight with few tiles in two slabs of 16: blocks for twice as many units (2,048 x
+    // 2,048 by 32 rows: 4.0 us against 5.4)
+    if (a.M <= 32 && (a.n_out + 15) / 16 <= llm_compute_units() / 2) return pick_mx4_tiles<1, 4, 4, EPI, NORM, OutT, X4>(a);
+    return pick_mx4_tiles<2, 4, 3, EPI, NORM, OutT, X4>(a);
+  }
   return LLM_ERR_ARG;
 }
 

@@ -91,7 +91,7 @@ class Mx4Matrix:
 class Mx4Ops:
     """The operations of ``HipOps`` on matrices in MXFP4."""
 
-    MX4_ROWS = 32           # most rows that go to the product for few rows wherever W goes
+    MX4_ROWS = 32           # most rows that go to the product for few rows, but for the widest weights and the smallest
     MX4_PLANS = 4096        # launch plans kept, by sizes
 
     # ---- conversions
@@ -157,13 +157,17 @@ class Mx4Ops:
 
     # ---- products
     def _mx4_few(self, m, n_out, four):
-        """Whether the product goes to the kernel for few rows: up to MX4_ROWS, and up to twice as many
-        where W has few tiles of outputs, so that the other would leave units idle (us, 64 rows,
-        that kernel against this: bfloat16, K 2,048, 2,048 outputs 5.5 against 10.4, but K 4,096,
-        6,144 outputs 17.5 against 17.8 and K 14,336, 4,096 outputs 36 against 22; MXFP4, in the
-        same order, 3.6 against 6.2, 8.6 against 11.1 and 18.3 against 17.5)."""
+        """Whether the product goes to the kernel for few rows.  Up to 16 rows always.  Up to 32 unless W
+        has tiles of outputs for three blocks a compute unit, with which the other fills the units too
+        (gate and up of 4,096 x 14,336: 32 to 35 us against 23).  Up to 64 where W has so few tiles that
+        the other would leave units idle (us, 64 rows, that kernel against this: bfloat16, K 2,048, 2,048
+        outputs 5.5 against 10.4, but K 4,096, 6,144 outputs 17.5 against 17.8 and K 14,336, 4,096
+        outputs 36 against 22; MXFP4, in the same order, 3.6 against 6.2, 8.6 against 11.1 and 18.3
+        against 17.5)."""
         tiles = -(-n_out // TILE_ROWS)
-        return m <= self.MX4_ROWS or (m <= 2 * self.MX4_ROWS and 2 * tiles <= (3 if four else 1) * self.units)
+        if m <= self.MX4_ROWS:
+            return m <= TILE_ROWS or tiles < 3 * self.units
+        return m <= 2 * self.MX4_ROWS and 2 * tiles <= (3 if four else 1) * self.units
 
     # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, and the us
     # that 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much
