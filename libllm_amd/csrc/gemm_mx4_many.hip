@@ -63,30 +63,40 @@ __device__ __forceinline__ void lds_fill(uint32_t lds, const void* base, uint32_
                : "=&s"(m0_was) : "s"(lds), "v"(off), "s"(base) : "memory");
 }
 
-template <bool X4, int NBUF, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
+// Sizes of a form.  A tile of K is UPT units of 128 elements, NBUF of them are held in LDS.  EARLY: with
+// few waves a unit nothing covers the latency of LDS; fragments are then read two steps ahead (into a second
+// set) instead of one, and the barrier of a tile lies a step earlier.  A buffer is filled again a tile
+// later than it could be: its reads are long over by then, and the barrier need not wait for those
+// under way.
+template <bool X4, int NBUF, bool EARLY, int WM, int WN, int MTW, int NTW>
+struct ManyShape {
+  static constexpr int UPT = X4 ? 2 : 1;
+  static constexpr int BM = WM * MTW * 16, BNT = WN * NTW;          // rows of X, tiles of W a block
+  static constexpr bool WL = X4 || NBUF > 2;                        // W's codes and scales go through LDS
+  static constexpr int XB = X4 ? BM * 64 * UPT : BM * 256;          // bytes of X's tile of K
+  static constexpr int BUF = XB + (X4 ? BNT * 1024 * UPT : WL ? BNT * 1024 : 0);
+  static constexpr int TPQ = 4 / UPT;                               // tiles of K a quad
+  static constexpr int FAR = EARLY ? NBUF - 1 : NBUF;               // tiles from the one at work to the one asked for
+  static constexpr int STILES = X4 ? BM / 16 + BNT : WL ? BNT : 0;  // tiles whose scales go through LDS: W's, then X's
+  static constexpr int SB = STILES * 256, NSB = (FAR + TPQ - 1) / TPQ;      // scales of a quad, quads held
+  static constexpr int BYTES = NBUF * BUF + NSB * SB;
+};
+
+template <bool X4, int NBUF, bool EARLY, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char lds[];
+  typedef ManyShape<X4, NBUF, EARLY, WM, WN, MTW, NTW> Shape;
   constexpr int NW = WM * WN;
-  constexpr int BM = WM * MTW * 16, BNT = WN * NTW;         // rows of X, tiles of W a block
-  constexpr int STEPS = X4 ? 2 : 4;
-  constexpr int XB = X4 ? BM * 128 : BM * 256;              // bytes of X's tile of K
-  // With few waves a unit, nothing covers the latency of LDS: fragments are then read two steps ahead
-  // (into a second set) instead of one, and the barrier of a tile lies a step earlier.
-  constexpr bool EARLY = NBUF > 2;
-  // A buffer is then filled again a tile later than it could be: its reads are long over by then, and
-  // the barrier need not wait for those under way.
+  constexpr int BM = Shape::BM, BNT = Shape::BNT, XB = Shape::XB, BUF = Shape::BUF, STILES = Shape::STILES, SB = Shape::SB;
+  constexpr int FAR = Shape::FAR, NSB = Shape::NSB, TPQ = Shape::TPQ, UPT = Shape::UPT;
+  constexpr bool WL = Shape::WL;
+  constexpr int STEPS = X4 ? UPT : 4;                       // steps of matrix instructions a tile of K
   constexpr int AHEAD = EARLY ? 2 : 1, BSTEP = STEPS - AHEAD;
-  constexpr int FAR = EARLY ? NBUF - 1 : NBUF;              // tiles from the one at work to the one asked for
-  constexpr bool WL = X4 || NBUF > 2;                       // W's codes and scales go through LDS
-  constexpr int WB = X4 ? BNT * 2048 : WL ? BNT * 1024 : 0;
-  constexpr int BUF = XB + WB;
-  constexpr int STILES = X4 ? BM / 16 + BNT : WL ? BNT : 0; // tiles whose scales do: W's, then X's
-  constexpr int SB = STILES * 256;                          // scales of a quad
-  constexpr int TPQ = X4 ? 2 : 4;                           // tiles of K a quad
-  constexpr int NSB = NBUF > TPQ + 1 ? 4 : 2;               // quads of scales held
-  constexpr int TURNS = WL && TPQ > NBUF ? TPQ : NBUF;      // rounds after which all of these repeat
+  constexpr int TURNS = WL && TPQ > 2 ? TPQ : 2;            // rounds after which sets of registers and bytes of scales repeat
   constexpr int XF = XB / 1024 / NW, FILLS = BUF / 1024 / NW;       // loads of 1 KiB a wave and tile: X's, all
-  static_assert(XB % (1024 * NW) == 0 && BUF % (1024 * NW) == 0 && TURNS % 2 == 0, "every wave fills as much");
+  constexpr int XT = UPT * 1024;                            // bytes of a row tile of X, or a tile of W, in MXFP4
+  static_assert(XB % (1024 * NW) == 0 && BUF % (1024 * NW) == 0, "every wave fills as much");
+  static_assert(STEPS >= AHEAD && (STEPS * TURNS) % 2 == 0 && TURNS % TPQ == 0 || !WL, "the sets repeat");
   constexpr bool GATED = EPI == MM_EPI_GATED;
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 15, g = lane >> 4;
@@ -135,9 +145,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   for (int p = 0; p < FILLS; ++p) {
     const int c = p * NW + wave;                            // which KiB of the buffer
     if (X4) {                                               // (tile, unit) of X, then of W
-      const int t = c >> 1;
+      const int t = c / UPT;
       fill_base[p] = (p < XF ? a.xc + (size_t)min(m0 / 16 + t, (a.M - 1) / 16) * c_tile
-                             : a.wc + (size_t)w_tile(t - BM / 16) * c_tile) + (c & 1) * 1024;
+                             : a.wc + (size_t)w_tile(t - BM / 16) * c_tile) + (c % UPT) * 1024;
     } else {                                                // four rows of X; a tile of W
       fill_base[p] = p < XF ? (const uint8_t*)(a.X + (size_t)m0 * a.ldx) : a.wc + (size_t)w_tile(c - XB / 1024) * c_tile;
     }
@@ -156,14 +166,14 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     sc_base = (t < BNT ? a.ws + (size_t)w_tile(t) * s_tile
                        : a.xs + (size_t)min(m0 / 16 + t - BNT, (a.M - 1) / 16) * s_tile) + (lane & 15) * 16;
   }
-  const int n_kt = X4 ? (units + 1) / 2 : units;
-  // Tile kt of K into buffer `buf`; past the last tile the last one again, which nobody reads: the
+  const int n_kt = X4 ? (units + UPT - 1) / UPT : units;
+  // Tile kt of K into the buffer at `at`; past the last tile the last one again, which nobody reads: the
   // loop has no branch then, over which the compiler would move matrix instructions.
-  auto fill = [&](int kt, int buf, int p) MM_INLINE {
-    const uint32_t at = lds0 + buf * BUF + (p * NW + wave) * 1024;
+  auto fill = [&](int kt, uint32_t at, int p) MM_INLINE {
+    at += lds0 + (p * NW + wave) * 1024;
     const size_t k = min(kt, n_kt - 1);
     if (X4) {
-      lds_fill(at, fill_base[p] + k * 2048, lane16);
+      lds_fill(at, fill_base[p] + k * XT, lane16);
     } else if (p >= XF) {
       lds_fill(at, fill_base[p] + k * 1024, lane16);
     } else {                                                // (the offset made anew each time: held, it would cost a register a fill)
@@ -177,7 +187,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     if constexpr (WL) {
       uint32_t m0_was;
       asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, off\n\ts_mov_b32 m0, %0"
-                   : "=&s"(m0_was) : "s"(lds0 + NBUF * BUF + (q & (NSB - 1)) * SB + sc_wave * 1024),
+                   : "=&s"(m0_was) : "s"(lds0 + NBUF * BUF + (q % NSB) * SB + sc_wave * 1024),
                      "v"(sc_base + (size_t)min(q, quads - 1) * 256) : "memory");
     }
   };
@@ -189,30 +199,30 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     for (int mt = 0; mt < MTW; ++mt) acc[nt][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   // ---- fragments.  The matrix instructions of a step go by row tile of X: once a tile's are issued,
-  // its fragment of the next step is read into the same registers.  Addresses are kept few: the
-  // compiler would hold one for every read of the loop and run out of registers.
+  // its fragment of a later step is read into the same registers.  Addresses are kept few: the compiler
+  // would hold one for every read of the loop and run out of registers.
   typedef uint32_t u4_raw __attribute__((ext_vector_type(4)));
   Frag xf[AHEAD][MTW];
   Frag wf[2][X4 ? NTW : 1];
-  uint32_t sc[2][X4 ? (NTW + MTW) / 2 : 1];                 // scales of a tile of K: two bytes of two tiles a word
-  u4_raw wc[2][X4 ? 1 : NTW];                               // W's codes of a tile of K, and its scales
-  uint32_t wsc[2][X4 ? 1 : NTW];
-  const uint32_t x_lane = lds0 + wm * MTW * (X4 ? 2048 : 4096) + (X4 ? lane16 : r * 256 + ((g * 4) ^ r) * 16);
+  u4_raw wc[2][X4 ? 1 : NTW];                               // W's codes of a tile of K (and, from registers, its scales)
+  uint32_t wsc[2][X4 || WL ? 1 : NTW];
+  constexpr int NS = X4 ? NTW + MTW : WL ? NTW : 1;         // scales of a quad: W's tiles, then X's; and of the next
+  uint32_t sc[NS], sc_next[NS];
+  const uint32_t x_lane = lds0 + wm * MTW * (X4 ? XT : 4096) + (X4 ? lane16 : r * 256 + ((g * 4) ^ r) * 16);
   const uint32_t w_lane = lds0 + XB + lane16;
   typedef const __attribute__((address_space(3))) u4_raw* lds_u4;
-  typedef const __attribute__((address_space(3))) uint16_t* lds_u2;
-  typedef const __attribute__((address_space(3))) uint8_t* lds_u1;
+  typedef const __attribute__((address_space(3))) uint32_t* lds_u1;
   typedef const __attribute__((address_space(1))) u4_raw* global_u4;
   typedef const __attribute__((address_space(1))) uint32_t* global_u1;
-  auto plus = [&](uint32_t lane_at, int by) MM_INLINE {
+  auto plus = [&](uint32_t lane_at, uint32_t by) MM_INLINE {
     uint32_t at;
     asm volatile("v_add_u32 %0, %1, %2" : "=v"(at) : "s"(by), "v"(lane_at));
     return at;
   };
-  auto x_step = [&](int buf, int step) MM_INLINE {                    // (piece 4 g + step of row r lies at its xor with r)
+  auto x_step = [&](uint32_t buf, int step) MM_INLINE {     // (piece 4 g + step of row r lies at its xor with r)
     uint32_t at = x_lane;
     if constexpr (!X4) asm volatile("v_xor_b32 %0, %1, %2" : "=v"(at) : "s"(step * 16), "v"(x_lane));
-    return plus(at, buf * BUF + (X4 ? step * 1024 : 0));
+    return plus(at, buf + (X4 ? step * 1024 : 0));
   };
   auto lds_read = [&](uint32_t at) MM_INLINE {
     const u4_raw v = *(lds_u4)(uintptr_t)at;
@@ -220,16 +230,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     f.u = make_uint4(v.x, v.y, v.z, v.w);
     return f;
   };
-  auto read_x = [&](uint32_t at, int mt) MM_INLINE { return lds_read(at + mt * (X4 ? 2048 : 4096)); };
-  auto read_w = [&](uint32_t at, int nt) MM_INLINE { return lds_read(at + wave_tile(nt) * 2048); };
-  auto read_scales = [&](uint32_t at, int i, uint32_t& lo, uint32_t& hi) MM_INLINE {      // word i: tiles 2 i and 2 i + 1, W's first
-    const int t0 = 2 * i < NTW ? wave_tile(2 * i) : BNT + wm * MTW + 2 * i - NTW;
-    const int t1 = 2 * i < NTW ? wave_tile(2 * i + 1) : t0 + 1;
-    lo = *(lds_u2)(uintptr_t)(at + t0 * 256);
-    hi = *(lds_u2)(uintptr_t)(at + t1 * 256);
-  };
+  auto read_x = [&](uint32_t at, int mt) MM_INLINE { return lds_read(at + mt * (X4 ? XT : 4096)); };
+  auto read_w = [&](uint32_t at, int nt) MM_INLINE { return lds_read(at + wave_tile(nt) * XT); };
   auto read_codes = [&](uint32_t at, int nt) MM_INLINE { return *(lds_u4)(uintptr_t)(at + wave_tile(nt) * 1024); };
-  auto read_scale = [&](uint32_t at, int nt) MM_INLINE { return (uint32_t) * (lds_u1)(uintptr_t)(at + wave_tile(nt) * 256); };
+  auto read_scale = [&](uint32_t at, int i) MM_INLINE {
+    return *(lds_u1)(uintptr_t)(at + (i < NTW ? wave_tile(i) : BNT + wm * MTW + i - NTW) * 256);
+  };
   auto load_w = [&](int kt, int set) MM_INLINE {
 #pragma unroll
     for (int nt = 0; nt < NTW; ++nt) {
@@ -244,7 +250,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
 
   each<FAR>([&](auto b) MM_INLINE {
     if (b % TPQ == 0) fill_scales(b / TPQ);
-    each<FILLS>([&](auto p) MM_INLINE { fill(b, b, p); });
+    each<FILLS>([&](auto p) MM_INLINE { fill(b, b * BUF, p); });
   });
   // (the compiler is told that it has W's codes: else it would wait for them, and with them for every
   // load into LDS behind them, inside the loop)
@@ -265,7 +271,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
       asm volatile("" ::: "memory");
     } else {
       asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(LEFT) : "memory");
-      __syncthreads();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
     }
   };
   arrived(std::integral_constant<int, FAR - 1>{});
@@ -274,53 +281,48 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     const uint32_t x_at = x_step(0, ahead);
 #pragma unroll
     for (int mt = 0; mt < MTW; ++mt) xf[ahead][mt] = read_x(x_at, mt);
-  }
-  if constexpr (X4) {
-#pragma unroll
-    for (int ahead = 0; ahead < AHEAD; ++ahead)
+    if constexpr (X4) {
 #pragma unroll
       for (int nt = 0; nt < NTW; ++nt) wf[ahead][nt] = read_w(w_lane + ahead * 1024, nt);
-#pragma unroll
-    for (int i = 0; i < (NTW + MTW) / 2; ++i) {
-      uint32_t lo, hi;
-      read_scales(lds0 + NBUF * BUF + lane4, i, lo, hi);
-      sc[0][i] = lo | hi << 16;
     }
-  } else if constexpr (WL) {
+  }
+  if constexpr (WL) {
 #pragma unroll
-    for (int nt = 0; nt < NTW; ++nt) {
-      wc[0][nt] = read_codes(w_lane, nt);
-      wsc[0][nt] = read_scale(lds0 + NBUF * BUF + lane4, nt);
+    for (int i = 0; i < NS; ++i) sc[i] = read_scale(lds0 + NBUF * BUF + lane4, i);
+    if constexpr (!X4) {
+#pragma unroll
+      for (int nt = 0; nt < NTW; ++nt) wc[0][nt] = read_codes(w_lane, nt);
     }
   }
 
-  // One tile of K, the turn-th of TURNS; CUR: which set of scales (or codes of W) is its own.
-  auto round = [&](int kt, auto turn) MM_INLINE {
-    constexpr int TURN = decltype(turn)::value, CUR = TURN & 1, NEXT = CUR ^ 1;
-    uint32_t sc_lo[(NTW + MTW) / 2], sc_hi[(NTW + MTW) / 2];
+  // One tile of K, the turn-th of TURNS: it lies in the buffer at `here`, the next one in that at `there`, and
+  // the one FAR tiles on goes into that at `to`.
+  auto round = [&](int kt, auto turn, uint32_t here, uint32_t there, uint32_t to) MM_INLINE {
+    constexpr int TURN = decltype(turn)::value, CUR = TURN & 1, NEXT = CUR ^ 1, IN_QUAD = TURN % TPQ;
+    constexpr bool NEW_SCALES = WL && IN_QUAD == TPQ - 1;   // the next tile's are another quad's
     if constexpr (!WL) load_w(min(kt + 1, n_kt - 1), NEXT);
     each<STEPS>([&](auto step) MM_INLINE {
-      constexpr int S = decltype(step)::value, SET = S & 1;
+      constexpr int S = decltype(step)::value, SET = (TURN * STEPS + S) & 1;
       constexpr int XS = EARLY ? SET : 0;
-      constexpr bool BORDER = S == BSTEP;                                    // from here on everything read is the next tile's
-      constexpr int RBUF = (TURN + (S >= BSTEP)) % NBUF, RS = (S + AHEAD) % STEPS;      // where the fragments to be read lie
+      constexpr bool BORDER = S == BSTEP;                   // from here on everything read is the next tile's
+      constexpr int RS = (S + AHEAD) % STEPS;               // the step whose fragments are read
       if constexpr (BORDER) {
         __builtin_amdgcn_sched_barrier(0);
         if constexpr (!WL) have_w(NEXT);
         arrived(std::integral_constant<int, FAR - 2>{});
       }
-      const uint32_t x_at = x_step(RBUF, RS);
+      const uint32_t from = S >= BSTEP ? there : here;
+      const uint32_t x_at = x_step(from, RS);
       uint32_t w_at = 0, s_at = 0;
       Frag w[X4 ? 1 : NTW];
-      if constexpr (WL) {
-        if constexpr (X4 || BORDER) w_at = plus(w_lane, RBUF * BUF + (X4 ? RS * 1024 : 0));
-        if constexpr (BORDER)
-          s_at = plus(lane4, lds0 + NBUF * BUF + (((kt + 1) / TPQ) & (NSB - 1)) * SB + (TURN + 1) % TPQ * (X4 ? 2 : 1));
-      }
+      if constexpr (X4 || (WL && BORDER)) w_at = plus(w_lane, from + (X4 ? RS * 1024 : 0));
+      if constexpr (NEW_SCALES && BORDER) s_at = plus(lane4, lds0 + NBUF * BUF + ((kt + 1) / TPQ % NSB) * SB);
       if constexpr (!X4) {
-        const int sh = WL ? 0 : 8 * (kt & 3);
 #pragma unroll
-        for (int nt = 0; nt < NTW; ++nt) w[nt] = mx4_widen(wc[CUR][nt][S], mx4_scale((wsc[CUR][nt] >> sh) & 255u));
+        for (int nt = 0; nt < NTW; ++nt) {
+          const uint32_t e = WL ? sc[nt] >> (8 * IN_QUAD) : wsc[CUR][nt] >> (8 * (kt & 3));
+          w[nt] = mx4_widen(wc[CUR][nt][S], mx4_scale(e & 255u));
+        }
       }
       each<MTW>([&](auto mtc) MM_INLINE {
         constexpr int MT = decltype(mtc)::value;
@@ -329,13 +331,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
         if constexpr (BORDER) {
           if (MT == 0 && (TURN + FAR) % TPQ == 0) fill_scales((kt + FAR) / TPQ);
 #pragma unroll
-          for (int p = FILLS * MT / MTW; p < FILLS * (MT + 1) / MTW; ++p) fill(kt + FAR, (TURN + FAR) % NBUF, p);
+          for (int p = FILLS * MT / MTW; p < FILLS * (MT + 1) / MTW; ++p) fill(kt + FAR, to, p);
         }
         each<NTW>([&](auto ntc) MM_INLINE {
           constexpr int NT = decltype(ntc)::value;
           if constexpr (X4)
-            acc[NT][MT] = mx4_mfma<(NT & 1) * 2 + S, (MT & 1) * 2 + S>(wf[SET][NT].u, sc[CUR][NT / 2], xf[XS][MT].u,
-                                                                       sc[CUR][NTW / 2 + MT / 2], acc[NT][MT]);
+            acc[NT][MT] = mx4_mfma<IN_QUAD * UPT + S, IN_QUAD * UPT + S>(wf[SET][NT].u, sc[NT], xf[XS][MT].u, sc[NTW + MT], acc[NT][MT]);
           else
             acc[NT][MT] = mfma_bf16(w[NT], xf[XS][MT], acc[NT][MT]);
         });
@@ -350,31 +351,34 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
 #pragma unroll
             for (int nt = 0; nt < NTW; ++nt) wf[SET][nt] = read_w(w_at, nt);
           }
-          if constexpr (BORDER) {
-            constexpr int NS = (NTW + MTW) / 2;
-#pragma unroll
-            for (int i = NS * MT / MTW; i < NS * (MT + 1) / MTW; ++i) read_scales(s_at, i, sc_lo[i], sc_hi[i]);
-          }
         } else if constexpr (WL && BORDER) {
 #pragma unroll
-          for (int nt = NTW * MT / MTW; nt < NTW * (MT + 1) / MTW; ++nt) {
-            wc[NEXT][nt] = read_codes(w_at, nt);
-            wsc[NEXT][nt] = read_scale(s_at, nt);
-          }
+          for (int nt = NTW * MT / MTW; nt < NTW * (MT + 1) / MTW; ++nt) wc[NEXT][nt] = read_codes(w_at, nt);
+        }
+        if constexpr (NEW_SCALES && BORDER) {
+#pragma unroll
+          for (int i = NS * MT / MTW; i < NS * (MT + 1) / MTW; ++i) sc_next[i] = read_scale(s_at, i);
         }
       });
     });
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (X4) {
+    if constexpr (NEW_SCALES) {
 #pragma unroll
-      for (int i = 0; i < (NTW + MTW) / 2; ++i) sc[NEXT][i] = sc_lo[i] | sc_hi[i] << 16;
+      for (int i = 0; i < NS; ++i) sc[i] = sc_next[i];
     }
   };
-  static_assert(STEPS % 2 == 0, "a tile of K ends on the set of W's fragments that it began with");
+  // where tile kt + FAR goes: FAR is the number of buffers, or one less
+  uint32_t here = 0, there = NBUF > 1 ? BUF : 0, to = FAR % NBUF * BUF;
+  auto turn_over = [&](int kt, auto turn) MM_INLINE {
+    round(kt, turn, here, there, to);
+    here = there;
+    there = there == (NBUF - 1) * BUF ? 0 : there + BUF;
+    to = to == (NBUF - 1) * BUF ? 0 : to + BUF;
+  };
   int kt = 0;
-  for (; kt + TURNS <= n_kt; kt += TURNS) each<TURNS>([&](auto turn) MM_INLINE { round(kt + turn, turn); });
+  for (; kt + TURNS <= n_kt; kt += TURNS) each<TURNS>([&](auto turn) MM_INLINE { turn_over(kt + turn, turn); });
   each<TURNS - 1>([&](auto turn) MM_INLINE {
-    if (kt + turn < n_kt) round(kt + turn, turn);
+    if (kt + turn < n_kt) turn_over(kt + turn, turn);
   });
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");       // the last loads into LDS have landed too
 
@@ -464,15 +468,13 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
   }
 }
 
-template <bool X4, int NBUF, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
+template <bool X4, int NBUF, bool EARLY, int WM, int WN, int MTW, int NTW, int EPI, typename OutT>
 static int launch_mx4_many(Mx4ManyArgs a) {
-  constexpr int BM = WM * MTW * 16, BNT = WN * NTW, NW = WM * WN;
-  constexpr bool WL = X4 || NBUF > 2;                        // (sizes as in the kernel)
-  constexpr int BUF = X4 ? BM * 128 + BNT * 2048 : BM * 256 + (WL ? BNT * 1024 : 0);
-  constexpr int SB = (X4 ? BM / 16 + BNT : WL ? BNT : 0) * 256, NSB = NBUF > (X4 ? 2 : 4) + 1 ? 4 : 2;
+  typedef ManyShape<X4, NBUF, EARLY, WM, WN, MTW, NTW> Shape;
+  constexpr int BM = Shape::BM, BNT = Shape::BNT, NW = WM * WN;
   constexpr int OUT_NT = EPI == MM_EPI_GATED ? NTW / 2 : NTW;
   constexpr int TURN = NW * 16 * (OUT_NT * 32 + 16);
-  constexpr int HELD = NBUF * BUF + NSB * SB, LDS_BYTES = HELD > TURN ? HELD : TURN;
+  constexpr int LDS_BYTES = Shape::BYTES > TURN ? Shape::BYTES : TURN;
   static_assert(LDS_BYTES <= 160 * 1024, "shared memory of a unit");
   const int out_tiles = (a.n_out + 15) / 16, per = EPI == MM_EPI_GATED ? BNT / 2 : BNT;
   a.m_tiles = (a.M + BM - 1) / BM;
@@ -484,34 +486,43 @@ static int launch_mx4_many(Mx4ManyArgs a) {
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return LLM_ERR_LAUNCH;
   if (!asked[dev]) {
-    if (hipFuncSetAttribute((const void*)gemm_mx4_many_kernel<X4, NBUF, WM, WN, MTW, NTW, EPI, OutT>,
+    if (hipFuncSetAttribute((const void*)gemm_mx4_many_kernel<X4, NBUF, EARLY, WM, WN, MTW, NTW, EPI, OutT>,
                             hipFuncAttributeMaxDynamicSharedMemorySize, LDS_BYTES) != hipSuccess)
       return LLM_ERR_LAUNCH;
     asked[dev] = true;
   }
   const dim3 grid((unsigned)blocks, (a.quads + a.slice_quads - 1) / a.slice_quads);
-  gemm_mx4_many_kernel<X4, NBUF, WM, WN, MTW, NTW, EPI, OutT><<<grid, NW * 64, LDS_BYTES, a.stream>>>(a);
+  gemm_mx4_many_kernel<X4, NBUF, EARLY, WM, WN, MTW, NTW, EPI, OutT><<<grid, NW * 64, LDS_BYTES, a.stream>>>(a);
   return llm_launch_status();
 }
 
 // Forms: rows of X by rows of W a block.  0, 256 x 256: fewest bytes a product, one block a unit.  1,
-// 128 x 128 (MXFP4 rows only: in bfloat16 form 2 is as fast or faster at every size measured).  2,
-// 64 x 128: several blocks a unit, which cover each other's waits.  3, 64 x 128 with four tiles of K
-// held and fragments two steps ahead: for a block a unit or less, where a block waits for memory (1.5 us
+// 128 x 128 (MXFP4) or 128 x 256 (bfloat16, where three tiles of K fit): more blocks, for products that
+// would leave units idle in the last round (bfloat16, 4,096 rows, K 4,096, 6,144 outputs: 157 us against
+// 167).  2, 64 x 128: several blocks a unit, which cover each other's waits.  3, 64 x 128 with four tiles of
+// K held and fragments two steps ahead: for a block a unit or less, where a block waits for memory (1.5 us
 // from a weight that no cache holds).  In bfloat16 that form has eight waves (128 rows, K 4,096, 6,144
-// outputs, us: 19.6, by four waves 22.3, form 2 27.5).
+// outputs, us: 19.6, by four waves 22.3, form 2 22.9).
+// Left as they are, measured: four tiles of 128 elements instead of two of 256 in form 0 of MXFP4 (61.2 us
+// against 59.6 at 4,096 rows, K 4,096, 6,144 outputs), and the widening taken out of form 0 in bfloat16
+// (no change): neither latency nor the vector units bound the large products.
 #define MM_FORMS 4
 template <bool X4, int EPI, typename OutT>
 static int pick_mx4_many(const Mx4ManyArgs& a, int form) {
-  switch (form) {
-    case 0: return launch_mx4_many<X4, 2, 2, 4, 8, 4, EPI, OutT>(a);
-    case 1:
-      if constexpr (X4) return launch_mx4_many<X4, 2, 2, 2, 4, 4, EPI, OutT>(a);
-      break;
-    case 2: return launch_mx4_many<X4, 2, 1, 4, 4, 2, EPI, OutT>(a);
-    case 3:
-      if constexpr (X4) return launch_mx4_many<X4, 4, 1, 4, 4, 2, EPI, OutT>(a);
-      else return launch_mx4_many<X4, 4, 2, 4, 2, 2, EPI, OutT>(a);
+  if constexpr (X4) {
+    switch (form) {
+      case 0: return launch_mx4_many<true, 2, false, 2, 4, 8, 4, EPI, OutT>(a);
+      case 1: return launch_mx4_many<true, 2, false, 2, 2, 4, 4, EPI, OutT>(a);
+      case 2: return launch_mx4_many<true, 2, false, 1, 4, 4, 2, EPI, OutT>(a);
+      case 3: return launch_mx4_many<true, 4, true, 1, 4, 4, 2, EPI, OutT>(a);
+    }
+  } else {
+    switch (form) {
+      case 0: return launch_mx4_many<false, 2, false, 2, 4, 8, 4, EPI, OutT>(a);
+      case 1: return launch_mx4_many<false, 3, false, 2, 4, 4, 4, EPI, OutT>(a);
+      case 2: return launch_mx4_many<false, 2, false, 1, 4, 4, 2, EPI, OutT>(a);
+      case 3: return launch_mx4_many<false, 4, true, 2, 4, 2, 2, EPI, OutT>(a);
+    }
   }
   return LLM_ERR_ARG;
 }

@@ -174,7 +174,8 @@ class Mx4Ops:
     # again for every four).  Measured over 2,048 to 14,336 elements of K, 33 to 4,096 rows, 2,048 to
     # 28,672 outputs; the forms' times cross where this says within a tenth.
     _MX4_FORMS = {
-        False: ((0, 256, 256, (2.7, 5.4, 8.1, 10.8)), (2, 64, 128, (0.71, 1.0, 1.43, 1.75)),
+        False: ((0, 256, 256, (2.7, 5.4, 8.1, 10.8)), (1, 128, 256, (1.45, 2.8, 4.2, 5.6)),
+                (2, 64, 128, (0.71, 1.0, 1.43, 1.75)),
                 (3, 64, 128, (0.58, 1.15, 1.75, 2.3))),
         True: ((0, 256, 256, (0.94, 1.88, 2.82, 3.76)), (1, 128, 128, (0.49, 0.63, 1.14, 1.33)),
                (2, 64, 128, (0.38, 0.44, 0.72, 0.85)), (3, 64, 128, (0.26, 0.52, 0.78, 1.04))),
@@ -196,7 +197,7 @@ class Mx4Ops:
                 a_unit = -(-blocks * ks // self.units)
                 cost = min(4 * per, all_units) * (times[3] * ((a_unit - 1) // 4) + times[(a_unit - 1) % 4])
                 if ks > 1:
-                    cost += 3.0 + ks * m * n * 8 / 4e6
+                    cost += 5.0 + ks * m * n * 8 / 3e6
                 if best is None or cost < best[0]:
                     best = (cost, form, ks)
         return best[1:]

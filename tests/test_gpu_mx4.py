@@ -80,6 +80,12 @@ def weight(n, k, seed):
     return codes, scales, values(codes, scales)
 
 
+def held(n, k, seed):
+    codes, scales, w = weight(n, k, seed)
+    packed, s = file_form(codes, scales)
+    return packed, s, w
+
+
 def bound(x, w, k, dtype):
     """What a product summed in 32 bits may be off by, per element.  Products of bfloat16 and MXFP4
     numbers (8 and 2 bits) are exact in 32 bits; k of them are added, in whatever order, by at most
@@ -270,6 +276,34 @@ def test_gated(ops, m, inter, k, four, act):
     assert (np.abs(got.double().cpu().numpy() - want) <= lim).all()
 
 
+FORMS = {False: (0, 1, 2, 3), True: (0, 1, 2, 3)}
+
+
+@pytest.mark.parametrize("four,form", [(f, i) for f in (False, True) for i in FORMS[f]])
+@pytest.mark.parametrize("m,n,k,ks", [(1, 16, 100, 1), (70, 130, 128, 1), (260, 300, 700, 1), (300, 520, 1500, 2),
+                                      (257, 272, 2600, 3), (40, 2064, 4200, 9), (530, 80, 3000, 1)])
+def test_every_form_of_the_product_for_many_rows(ops, monkeypatch, m, n, k, ks, four, form):
+    """At sizes that fill no block, with K of less than a tile, of odd numbers of tiles, and in slices of
+    which the last is short; plain, with a bias, and gated."""
+    monkeypatch.setattr(ops, "_mx4_plan", lambda *sizes: (form, ks))
+    x, b = normal((m, k), m + k, dtype=torch.bfloat16), normal((n,), 3)
+    packed, s, w = held(n, k, n + k)
+    q = ops.mx4_from_codes(packed.cuda(), s.cuda(), k)
+    rows = ops.quantize_mx4(x.cuda()) if four else x.cuda()
+    xd = values(*quantise(x.double().numpy())) if four else x.double().numpy()
+    y, lim = xd @ w.T, bound(xd, w, k, torch.float32)
+    got = ops.linear(rows, q, b.cuda(), torch.float32).double().cpu().numpy()
+    more = 2 * HALF_F32 * (np.abs(y) + np.abs(b.double().numpy()))
+    assert (np.abs(got - (y + b.double().numpy())) <= lim + more).all()
+    out = ops.linear(rows, q, None, torch.bfloat16).double().cpu().numpy()
+    assert (np.abs(out - y) <= bound(xd, w, k, torch.bfloat16)).all()
+    if n % 32 == 0:
+        sw = ops.linear_swiglu(rows, q).double().cpu().numpy()
+        g, u, dg, du = y[:, :n // 2], y[:, n // 2:], lim[:, :n // 2], lim[:, n // 2:]
+        ls = 1.2 * dg * (np.abs(u) + du) + (np.abs(g) + dg) * du + 2.0 ** -16 * np.abs(g) * np.abs(u)
+        assert (np.abs(sw - gate("silu", g, u)) <= ls + HALF_BF16 * (np.abs(gate("silu", g, u)) + ls) + 1e-38).all()
+
+
 def test_a_row_is_the_same_whatever_the_batch(ops):
     """Up to 32 rows, which one kernel takes."""
     x = normal((32, 1056), 8, dtype=torch.bfloat16).cuda()
@@ -403,12 +437,6 @@ def test_on_another_stream(ops):
 
 
 # ------------------------------------------------------------------------------- as a layer uses them
-def held(n, k, seed):
-    codes, scales, w = weight(n, k, seed)
-    packed, s = file_form(codes, scales)
-    return packed, s, w
-
-
 @pytest.mark.parametrize("m,n,k", [(1, 64, 96), (3, 77, 200), (16, 2048, 520), (20, 48, 1000), (32, 100, 64),
                                    (50, 4112, 136), (70, 64, 2100), (140, 96, 5000)])
 def test_added_into_the_stream(ops, m, n, k):

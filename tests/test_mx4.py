@@ -54,7 +54,7 @@ def test_plans_are_launches_the_kernels_take():
         if form < 0:
             assert ks == 1 and m <= 2 * ops.MX4_ROWS
             continue
-        assert form in ((0, 1, 2, 3) if four else (0, 2, 3))
+        assert form in (0, 1, 2, 3)
         quads = -(-k // 512)
         per = -(-quads // ks)
         assert -(-quads // per) == ks                    # no slice is empty
