@@ -58,11 +58,10 @@ class Mx4Matrix:
     def _new(cls, rows, width, device):
         """Room for a matrix: one allocation, the codes first."""
         q = cls.__new__(cls)
-        codes, scales = tiled_sizes(rows, width)
-        both = torch.empty(codes + scales, dtype=torch.uint8, device=device)
-        q.shape, q.device, q._storage = (rows, width), device, both
-        q.codes_ptr = both.data_ptr()
-        q.scales_ptr = q.codes_ptr + codes
+        cells = -(-rows // TILE_ROWS) * -(-width // QUAD)
+        q._storage = both = torch.empty(cells * 4352, dtype=torch.uint8, device=device)
+        q.shape, q.device, q.codes_ptr = (rows, width), device, both.data_ptr()
+        q.scales_ptr = q.codes_ptr + cells * 4096
         return q
 
     @property
@@ -150,6 +149,8 @@ class Mx4Ops:
 
     def _matrix(self, x, what):
         """A matrix on the device with contiguous rows."""
+        if x.dim() == 2 and x.is_contiguous() and x.device == self.device:
+            return
         if x.device != self.device:
             raise KernelError("%s lies on %s, not on %s" % (what, x.device, self.device))
         if x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < x.shape[1]):
@@ -216,21 +217,21 @@ class Mx4Ops:
 
     def _mx4_rows(self, x, k, piece):
         """bfloat16 rows for a kernel that reads ``piece`` elements of them at a time: ``x`` itself, or a
-        padded copy where its length, distance or address does not allow that."""
+        padded copy where its length, distance or address does not allow that; with its address and
+        the distance of its rows."""
         at = x.data_ptr()
-        if (x.dtype is torch.bfloat16 and x.device == self.device and x.dim() == 2 and x.is_contiguous()
-                and k % piece == 0 and at % 16 == 0):
-            return x, k
+        if x.dtype is torch.bfloat16 and k % piece == 0 and at % 16 == 0 and x.is_contiguous() and x.device == self.device:
+            return x, at, k
         if x.dtype != torch.bfloat16:
             raise KernelError("linear: an MXFP4 weight takes rows in bfloat16 or MXFP4, not %s" % (x.dtype,))
         self._matrix(x, "linear input")
         ld = max(x.stride(0), k)
         if k % piece == 0 and ld % piece == 0 and at % 16 == 0:
-            return x, ld
+            return x, at, ld
         ldp = -(-k // piece) * piece
         padded = torch.empty((x.shape[0], ldp), dtype=torch.bfloat16, device=self.device)
         self._launch("llm_pad_rows", at, ld, padded.data_ptr(), x.shape[0], k, ldp)
-        return padded, ldp
+        return padded, padded.data_ptr(), ldp
 
     def _mx4_product(self, x, w, n_out, out_dtype, epilogue, bias=None, stack=False):
         """The product of ``x`` (a matrix, MXFP4 rows, or a record of normed rows whose norm is
@@ -238,26 +239,27 @@ class Mx4Ops:
         unadded, ``[slices, m, n]`` in 32 bits."""
         self._mx4(w, "the weight")
         n, k = w.shape
-        pre = getattr(x, "pre", None)
-        m, k2 = pre.raw.shape if pre is not None else x.shape
+        four, ssq, eps = False, None, 0.0
+        if not isinstance(x, torch.Tensor):
+            if isinstance(x, Mx4Matrix):
+                self._mx4(x, "linear input")
+                four = True
+            else:
+                x, ssq, eps = x.pre.raw, x.pre.ssq.data_ptr(), x.pre.eps
+        m, k2 = x.shape
         if k != k2:
             raise KernelError("linear: x is [%d, %d] but the weight is [%d, %d]" % (m, k2, n, k))
         code = self._dtype_code(out_dtype)
         bptr = None if bias is None else self._dev(bias, "bias", torch.float32, (n,))
         if m == 0:
             return torch.empty((m, n_out), dtype=out_dtype, device=self.device)
-        four = isinstance(x, Mx4Matrix)
-        form, ks = self._mx4_plan(m, n, n_out, k, four)
+        form, ks = self._mx4_plans.get((m, n, n_out, k, four)) or self._mx4_plan(m, n, n_out, k, four)
         piece = 8 if form < 0 else 128
-        ssq, eps = None, 0.0
         if four:
-            self._mx4(x, "linear input")
             xp, xs, ldx = x.codes_ptr, x.scales_ptr, 0
         else:
-            if pre is not None:
-                x, ssq, eps = pre.raw, pre.ssq.data_ptr(), pre.eps
-            x, ldx = self._mx4_rows(x, k, piece)
-            xp, xs = x.data_ptr(), None
+            x, xp, ldx = self._mx4_rows(x, k, piece)
+            xs = None
         kp = -(-k // piece) * piece         # (where rows were padded, their length: the weight's codes there are zero)
         wp, ws = w.codes_ptr, w.scales_ptr
         if ks == 1:
@@ -281,8 +283,9 @@ class Mx4Ops:
     def _mx4_input(self, x, w):
         """``x`` for a product with ``w``: a record of normed rows goes in as it is where the product before
         has prepared its norm and the product for few rows takes it, else the norm kernel runs."""
-        pre = getattr(x, "pre", None)
-        if pre is not None and pre.raw.shape[0] <= self.ACCUM_ROWS and w.shape[1] == pre.raw.shape[1]:
+        if isinstance(x, (torch.Tensor, Mx4Matrix)):
+            return x
+        if x.pre is not None and x.pre.raw.shape[0] <= self.ACCUM_ROWS and w.shape[1] == x.pre.raw.shape[1]:
             return x
         return self._materialise(x, torch.bfloat16)
 
@@ -291,21 +294,21 @@ class Mx4Ops:
         the other returns the product, or its slices of K, for the norm that comes next to add."""
         x = self._mx4_input(x, w)
         n, k = w.shape
-        if residual is None or bias is not None or isinstance(x, Mx4Matrix) or getattr(x, "pre", None) is not None:
+        if residual is None or bias is not None or not isinstance(x, torch.Tensor):
             return self._mx4_product(x, w, n, out_dtype, self._EPI_NONE, bias, residual is not None)
         m = x.shape[0]
         if m == 0 or x.shape[1] != k or self._mx4_plan(m, n, n, k, False)[0] >= 0:
             return self._mx4_product(x, w, n, out_dtype, self._EPI_NONE, None, True)
         self._mx4(w, "the weight")
         self._dev(residual, "residual stream", torch.float32, (m, n))
-        x, ldx = self._mx4_rows(x, k, 8)
+        x, xp, ldx = self._mx4_rows(x, k, 8)
         record, nw, raw, ssq = None, None, None, None
         if then_norm is not None and self.fold_norms and m <= self.ACCUM_ROWS and n % 16 == 0:
             weight, eps = then_norm
             nw = self._dev(weight, "norm weight", torch.float32, (n,))
             record = self._prenormed(m, n, weight, eps)
             raw, ssq = record.raw.data_ptr(), record.ssq.data_ptr()
-        self._launch("llm_gemm_mx4_rows", x.data_ptr(), None, ldx, w.codes_ptr, w.scales_ptr, None, residual.data_ptr(),
+        self._launch("llm_gemm_mx4_rows", xp, None, ldx, w.codes_ptr, w.scales_ptr, None, residual.data_ptr(),
                      self._EPI_ACCUM, self._dtype_code(torch.float32), m, n, -(-k // 8) * 8, nw, raw, ssq, None, 0.0)
         return record
 
@@ -331,20 +334,20 @@ class Mx4Ops:
         """The stacked projection with its rotation and cache write in one kernel, or None where the
         product for few rows does not take it."""
         x = self._mx4_input(x, w)
-        pre = getattr(x, "pre", None)
-        rows = pre.raw if pre is not None else x
-        if isinstance(rows, Mx4Matrix):
+        if isinstance(x, Mx4Matrix):
             return None, x
+        pre = None if isinstance(x, torch.Tensor) else x.pre
+        rows = x if pre is None else pre.raw
         m, k = rows.shape
         n = w.shape[0]
         if m == 0 or k != w.shape[1] or self._mx4_plan(m, n, n, k, False)[0] >= 0:
             return None, x
         self._mx4(w, "qkv weight")
-        rows, ldx = self._mx4_rows(rows, k, 8)
+        rows, xp, ldx = self._mx4_rows(rows, k, 8)
         cptr, sptr, bptr, kptr, vptr, tptr, stride = self._rope_operands("qkv_rope", cos, sin, rot_dim, bias, n, ctx, kv, write,
                                                                          n_kv, hd, torch.bfloat16)
         q = torch.empty((m, n_heads * hd), dtype=torch.bfloat16, device=self.device)
-        self._launch("llm_gemm_mx4_rows_rope", rows.data_ptr(), ldx, w.codes_ptr, w.scales_ptr, bptr, q.data_ptr(), m,
+        self._launch("llm_gemm_mx4_rows_rope", xp, ldx, w.codes_ptr, w.scales_ptr, bptr, q.data_ptr(), m,
                      -(-k // 8) * 8, n_heads, n_kv, hd, cptr, sptr, rot_dim, ctx.tok_pos.data_ptr(), ctx.tok_seq.data_ptr(),
                      ctx.seq_slot.data_ptr(), tptr, stride, kptr, vptr, 64, 1 if write else 0,
                      pre.ssq.data_ptr() if pre is not None else None, pre.eps if pre is not None else 0.0)

@@ -271,7 +271,7 @@ class HipOps(Mx4Ops):
 
     @staticmethod
     def _dtype_code(dtype):
-        return _code(dtype)
+        return _BF16 if dtype is torch.bfloat16 else _code(dtype)
 
     @staticmethod
     def _check(status: int, what: str):
