@@ -399,8 +399,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
       v[e] = acc[nt][mt][e];
       if (GATED) {
         const float gt = acc[nt][mt][e], up = acc[nt + NTW / 2 < NTW ? nt + NTW / 2 : nt][mt][e];
-        v[e] = a.act == LLM_ACT_SILU ? up * gt * __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.4426950408889634f * gt))
-                                     : llm_gated(a.act, gt, up);
+        v[e] = a.act == LLM_ACT_SILU ? up * (gt * __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.4426950408889634f * gt)))
+                                     : llm_gated(a.act, gt, up);      // (the order: mx4_gated)
       } else {
         v[e] += bias[nt][e];
       }
@@ -577,8 +577,8 @@ extern "C" int llm_gemm_mx4_many(const void* X, const void* xs, int ldx, const v
   return xs == nullptr ? mx4_many<false>(a, epilogue, out_dtype, form) : mx4_many<true>(a, epilogue, out_dtype, form);
 }
 
-// The slices' sums parts [n_parts, M, N], added in their order, plus bias or through the gate, to C of
-// out_dtype: four columns a thread (N and n_out multiples of 4), or one.
+// The slices' sums parts [n_parts, M, N] (or one product whose gate and up lie in no whole tiles), added
+// in their order, plus bias or through the gate, to C of out_dtype: four columns a thread (N and n_out multiples of 4), or one.
 template <int VEC, bool GATED, typename OutT>
 __global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__ parts, int n_parts, const float* bias,
                                                        OutT* __restrict__ C, size_t M, int N, int n_out, int act) {
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-    if (GATED) v[e] = llm_gated(act, v[e], u[e]);
+    if (GATED) v[e] = mx4_gated(act, v[e], u[e]);
     else if (bias != nullptr) v[e] += bias[n + e];
   }
   OutT* dst = C + m * n_out + n;

@@ -30,6 +30,12 @@ typedef float f32x2_raw __attribute__((ext_vector_type(2)));
 // is 2^-127 and 255 NaN (checked on the device, tests/test_gpu_mx4.py).
 __device__ __forceinline__ float mx4_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
+// The gate of the gated products, in 32 bits.  SiLU is finished before it meets the other factor: that
+// times the gate may overflow where the result does not (gate -1e20, up 1e20).
+__device__ __forceinline__ float mx4_gated(int act, float g, float u) {
+  return act == LLM_ACT_SILU ? u * (g / (1.0f + expf(-g))) : llm_gated(act, g, u);
+}
+
 // Eight codes, widened with their scale; exact (an element has two significant bits).
 __device__ __forceinline__ Frag mx4_widen(uint32_t codes, float scale) {
   union {

@@ -324,11 +324,13 @@ class Mx4Ops:
         if dtype == torch.bfloat16 and n // 2 % TILE_ROWS == 0:
             return self._mx4_product(x, w, n // 2, dtype, self._EPI_SWIGLU | (act << 4))
         # up's rows begin inside a tile, or the result is wanted in 32 bits: the product in 32 bits, then the gate
-        y = self._mx4_product(x, w, n, torch.float32, self._EPI_NONE)
-        if y.shape[0] == 0:
-            return torch.empty((0, n // 2), dtype=dtype, device=self.device)
-        out = self.silu_mul(y, activation)
-        return out if out.dtype == dtype else out.to(dtype)
+        code = self._dtype_code(dtype)
+        y = self._mx4_product(x, w, n, torch.float32, self._EPI_NONE, None, True)
+        out = torch.empty((y.shape[-2], n // 2), dtype=dtype, device=self.device)
+        if y.shape[-2]:
+            self._launch("llm_mx4_join", y.data_ptr(), y.shape[0] if y.dim() == 3 else 1, None, out.data_ptr(),
+                         self._EPI_SWIGLU | (act << 4), code, y.shape[-2], n)
+        return out
 
     def _qkv_rope_mx4(self, x, w, bias, n_heads, n_kv, hd, cos, sin, rot_dim, ctx, kv, write):
         """The stacked projection with its rotation and cache write in one kernel, or None where the

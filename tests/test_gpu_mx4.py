@@ -279,6 +279,30 @@ def test_gated(ops, m, inter, k, four, act):
 FORMS = {False: (0, 1, 2, 3), True: (0, 1, 2, 3)}
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,inter,k", [(1, 16, 32), (3, 33, 32), (24, 80, 64), (40, 112, 64), (70, 33, 1100), (300, 272, 64)])
+def test_gated_with_numbers_whose_product_overflows(ops, m, inter, k, out):
+    """Gates of -2^70 k and ups of 2^70 k, whose product 32 bits do not hold: SiLU of such a gate is zero,
+    and with it the result.  With up zero as well, and with small gates in every third column, ordinary ones."""
+    g, u = np.full(inter, -1.0), np.ones(inter)
+    u[1::5] = 0.0
+    g[::3] = 2.0 ** -72 / k
+    u[::3] = 2.0 ** -70 / k
+    # one number a row, at the exponent that its block's scale gives it: 4 2^(e - 2)
+    rows = torch.tensor(np.repeat(np.concatenate([g, u])[:, None], k, 1), dtype=torch.float32).cuda()
+    x = torch.full((m, k), 2.0 ** 70, dtype=torch.bfloat16).cuda()
+    w = ops.quantize_mx4(rows)
+    held = ops.dequantize_mx4(w, torch.float32).double().cpu().numpy().sum(1) * 2.0 ** 70
+    gs, us = held[:inter], held[inter:]
+    want = np.where(gs < -700, 0.0, gs / (1 + np.exp(-np.maximum(gs, -700)))) * us
+    got = ops.linear_swiglu(x, w, out).double().cpu().numpy()
+    assert got.shape == (m, inter)
+    half = HALF_BF16 if out == torch.bfloat16 else HALF_F32
+    # equal terms: at most k additions a sum; the exponential, the division and two products are a few
+    # units of 2^-24 each, taken for 16
+    assert (np.abs(got - want) <= (half + (2 * k * 2 + 16) * HALF_F32) * np.abs(want)).all()
+
+
 @pytest.mark.parametrize("four,form", [(f, i) for f in (False, True) for i in FORMS[f]])
 @pytest.mark.parametrize("m,n,k,ks", [(1, 16, 100, 1), (70, 130, 128, 1), (260, 300, 700, 1), (300, 520, 1500, 2),
                                       (257, 272, 2600, 3), (40, 2064, 4200, 9), (530, 80, 3000, 1)])
