@@ -168,10 +168,10 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* __restrict
 // Rows of K bfloat16 elements into rows of K rounded up to 8, the elements added zero: for the
 // products, which read 16 bytes at a time, where K or the address is no multiple of that.
 __global__ __launch_bounds__(256) void pad_rows_kernel(const bf16_t* __restrict__ X, size_t ldx,
-                                                       bf16_t* __restrict__ out, int K, int ldo) {
-  const size_t m = blockIdx.x;
-  for (int k = blockIdx.y * 256 + threadIdx.x; k < ldo; k += gridDim.y * 256)
-    out[m * ldo + k] = k < K ? X[m * ldx + k] : (bf16_t)0;
+                                                       bf16_t* __restrict__ out, int M, int K, int ldo) {
+  for (size_t m = blockIdx.x; m < (size_t)M; m += gridDim.x)
+    for (int k = blockIdx.y * 256 + threadIdx.x; k < ldo; k += gridDim.y * 256)
+      out[m * ldo + k] = k < K ? X[m * ldx + k] : (bf16_t)0;
 }
 
 static inline dim3 mx4_grid(int rows, int k) { return dim3(mx4_tiles(rows), mx4_quads(k)); }
@@ -236,6 +236,7 @@ extern "C" int llm_mx4_pack(const void* rows, size_t ldc, const void* row_scales
 extern "C" int llm_pad_rows(const void* X, size_t ldx, void* out, int M, int K, int ldo, hipStream_t stream) {
   if (M <= 0) return LLM_OK;
   if (K <= 0 || ldx < (size_t)K || ldo < K || X == nullptr || out == nullptr) return LLM_ERR_ARG;
-  pad_rows_kernel<<<dim3(M, (ldo + 2047) / 2048), 256, 0, stream>>>((const bf16_t*)X, ldx, (bf16_t*)out, K, ldo);
+  const dim3 grid(M < (1 << 16) ? M : 1 << 16, ldo < (1 << 19) ? (ldo + 2047) / 2048 : 256);
+  pad_rows_kernel<<<grid, 256, 0, stream>>>((const bf16_t*)X, ldx, (bf16_t*)out, M, K, ldo);
   return llm_launch_status();
 }

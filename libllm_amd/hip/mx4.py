@@ -92,12 +92,13 @@ class Mx4Ops:
 
     MX4_ROWS = 32           # most rows that go to the product for few rows, but for the widest weights and the smallest
     MX4_PLANS = 4096        # launch plans kept, by sizes
+    MX4_FAR = 1 << 22       # most elements between two rows in bfloat16 for the product for many rows: a block's offsets have 32 bits
 
     # ---- conversions
     def _mx4_empty(self, rows, width):
         if rows <= 0 or width <= 0:
             raise KernelError("an MXFP4 matrix has rows and columns, not [%d, %d]" % (rows, width))
-        if rows >= 1 << 30 or width > 65535 * QUAD:
+        if rows > 1 << 27 or width > 65535 * QUAD:          # (threads of a launch, blocks along the second axis of a grid)
             raise KernelError("an MXFP4 matrix of [%d, %d] is too large" % (rows, width))
         return Mx4Matrix._new(rows, width, self.device)
 
@@ -211,7 +212,8 @@ class Mx4Ops:
         if plan is None:
             if len(self._mx4_plans) >= self.MX4_PLANS:
                 self._mx4_plans.clear()
-            plan = (-1, 1) if self._mx4_few(m, n_out, four) else self._mx4_form(m, n, k, four)
+            few = self._mx4_few(m, n_out, four) or (k > self.MX4_FAR and not four)
+            plan = (-1, 1) if few else self._mx4_form(m, n, k, four)
             self._mx4_plans[key] = plan
         return plan
 
@@ -226,7 +228,7 @@ class Mx4Ops:
             raise KernelError("linear: an MXFP4 weight takes rows in bfloat16 or MXFP4, not %s" % (x.dtype,))
         self._matrix(x, "linear input")
         ld = max(x.stride(0), k)
-        if k % piece == 0 and ld % piece == 0 and at % 16 == 0:
+        if k % piece == 0 and ld % piece == 0 and at % 16 == 0 and ld <= (self.MX4_FAR if piece > 8 else 1 << 30):
             return x, at, ld
         ldp = -(-k // piece) * piece
         padded = torch.empty((x.shape[0], ldp), dtype=torch.bfloat16, device=self.device)

@@ -369,6 +369,28 @@ def test_rows_that_lie_apart_or_askew(ops):
         assert torch.equal(ops.linear(view, q, None, torch.float32), ops.linear(view.contiguous(), q, None, torch.float32))
 
 
+@pytest.mark.parametrize("far,k", [((1 << 22) + 512, 256), ((1 << 22) + 128, (1 << 22) + 128), ((1 << 22) + 8, 200)])
+def test_rows_that_lie_far_apart(ops, far, k):
+    """A block's rows, and a width, that the product for many rows cannot reach with 32-bit offsets: numbers
+    of -1, 0 and 1, whose sums 32 bits hold."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randint(-1, 2, (70, far), generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)[:, :k]
+    w = torch.randint(-1, 2, (32, k), generator=g, device="cuda", dtype=torch.int8).to(torch.bfloat16)
+    got = ops.linear(x, ops.quantize_mx4(w), None, torch.float32)
+    want = torch.zeros((70, 32), dtype=torch.float64, device="cuda")
+    for at in range(0, k, 1 << 18):
+        want += x[:, at:at + (1 << 18)].double() @ w[:, at:at + (1 << 18)].double().t()
+    assert torch.equal(got.double(), want)
+
+
+def test_many_rows_that_are_padded(ops):
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randint(-4, 5, (70001, 3), generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.tensor([[1.0, -2.0, 3.0], [0.5, 6.0, -4.0]], device="cuda")
+    got = ops.linear(x, ops.quantize_mx4(w), None, torch.float32)
+    assert torch.equal(got.double(), x.double() @ w.double().t())
+
+
 def test_no_rows(ops):
     q = ops.quantize_mx4(normal((32, 64), 1).cuda())
     none = torch.empty((0, 64), dtype=torch.bfloat16, device="cuda")
