@@ -37,7 +37,7 @@ def tiled_sizes(rows: int, width: int):
 
 class Mx4Matrix:
     """A matrix ``[rows, width]`` in MXFP4: ``codes`` and ``scales`` are flat uint8 tensors in the
-    order the matrix cores read them.  What ``HipOps.quantize_mx4`` and ``HipOps.mx4_from_codes``
+    order the matrix cores read them, zero where rows and columns are filled up.  What ``HipOps.quantize_mx4`` and ``HipOps.mx4_from_codes``
     return, and the products take as a weight, or on both sides."""
     dtype = "mxfp4"
     __slots__ = ("shape", "device", "codes_ptr", "scales_ptr", "_storage")

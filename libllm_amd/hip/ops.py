@@ -212,7 +212,7 @@ class HipOps(Mx4Ops):
 
     # ---- time per operation, behind a switch
     _TIMED = ("embed", "embed_prepared", "add_rmsnorm", "linear", "linear_swiglu", "silu_mul", "qkv_rope", "rope_kv_write",
-              "attention", "argmax", "sample")
+              "attention", "argmax", "sample", "quantize_mx4", "dequantize_mx4", "mx4_from_codes")
 
     def start_timing(self) -> None:
         """From now on every operation is bracketed by two events on its stream, and

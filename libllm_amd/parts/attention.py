@@ -108,6 +108,7 @@ class Attention(Mixer):
                 if bias is not None:
                     bias = bias[order].contiguous()
         self.qkv.bind(w, ops=ops)
+        w = w if self.qkv.weight is None else self.qkv.weight
         self.q_only.bind(w[:self.q_dim], ops=ops, like=self.qkv.prepared)    # the same storage
         self.bias = bias                                 # added inside the rotation kernel
         self.out.bind(tensors[s.o_name + ".weight"], ops=ops)

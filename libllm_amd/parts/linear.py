@@ -24,8 +24,10 @@ class Linear:
         assert tuple(weight.shape) == (self.out_features, self.in_features)
         if self.low_bit and getattr(ops, "weight_format", None) == "mxfp4":
             self.weight, self.bias = None, bias
-            whole = like is not None and self.out_features % 16 == 0
-            self.prepared = like.leading_rows(self.out_features) if whole else ops.quantize_mx4(weight)
+            if like is not None and self.out_features % 16 == 0:
+                self.prepared = like.leading_rows(self.out_features)
+            else:
+                self.prepared = ops.quantize_mx4(weight if weight.stride(-1) == 1 else weight.contiguous())
             return
         self.weight = weight if weight.stride(-1) == 1 else weight.contiguous()
         self.bias = bias

@@ -72,3 +72,31 @@ def test_engine_refuses_formats_it_cannot_hold(tmp_path):
     for kw in ({"weights": "fp4"}, {"weights": "mxfp4", "dtype": "float32"}, {"weights": "mxfp4"}):
         with pytest.raises(ConfigError):
             random_engine(cfg, ops=Ops(), max_tokens=64, **kw)
+
+
+def test_a_matrix_is_bound_once_whatever_its_order():
+    """Rows in a row for the quantiser, a transposed matrix too; the leading rows in the same storage where
+    they are whole tiles."""
+    from libllm_amd.parts.linear import Linear
+
+    class Quantised:
+        def __init__(self, w):
+            assert w.stride(-1) == 1
+            self.w = w
+
+        def leading_rows(self, rows):
+            return ("leading", rows)
+
+    class Ops:
+        weight_format = "mxfp4"
+        quantize_mx4 = staticmethod(Quantised)
+    w = torch.arange(12 * 40).reshape(12, 40).float()
+    whole = Linear(12, 40, low_bit=True)
+    whole.bind(w.t(), ops=Ops())
+    assert whole.weight is None and torch.equal(whole.prepared.w, w.t())
+    part = Linear(12, 32, low_bit=True)
+    part.bind(w.t()[:32], ops=Ops(), like=whole.prepared)
+    assert part.prepared == ("leading", 32)
+    part = Linear(12, 24, low_bit=True)
+    part.bind(w.t()[:24], ops=Ops(), like=whole.prepared)
+    assert torch.equal(part.prepared.w, w.t()[:24])
