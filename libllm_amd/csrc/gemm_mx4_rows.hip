@@ -243,7 +243,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
 #pragma unroll
       for (int j = 0; j < RPR; ++j) {
         float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
+#pragma unroll 8                                          // (sixteen at once would not fit in the registers)
         for (int w = 0; w < WAVES; ++w) {
           const float4 p = *reinterpret_cast<const float4*>(red + w * RED + ((j * MT + mt) * 64 + lane) * 4);
           s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
@@ -298,32 +298,37 @@ static int launch_mx4_rows(const Mx4Args& a) {
 // where there are tiles of outputs for half of the compute units at most, 8 up to one a unit, else 4,
 // whose longer runs overlap better (us, 4 / 8 / 16 waves: 2,048 x 2,048 by 16 rows 4.6 / 4.6 / 3.9;
 // 14,336 x 4,096 by one row 9.7 / 8.6 / 8.8; 4,096 x 6,144 by 16 rows 9.6 / 11.6 / 11.2; gate and up
-// of 4,096 x 14,336 by 8 rows 20.2 / 26.1 / 28.5).  Two tiles of outputs a wave halve what a block
-// reads of X: from 9 rows on, where tiles are many (that gate and up: 23.0 against 24.1 us by 16 rows,
-// but 17.9 against 16.3 by one).
-template <int MT, int XQ, int STAGES, int EPI, bool NORM, typename OutT, bool X4>
+// of 4,096 x 14,336 by 8 rows 20.2 / 26.1 / 28.5).  Where several blocks fall to a unit, few registers
+// count for more than units in flight, since then they run at once: 3 units, from 9 rows on 2, where
+// there are tiles for three blocks a unit 1 (gate and up of 4,096 x 14,336, us by 8 / 16 rows: 4 units
+// 19.5 / 22.7, 3 units 16.7 / 21.0).  From 9 rows on a wave then takes two tiles of outputs, which
+// halves what a block reads of X (4,096 x 6,144 by 16 rows, 2 units: 7.1 us against 8.3 by one tile; that
+// gate and up by 16 / 32 rows, 1 unit: 17.6 / 22.7 against 21.0 / 27.9); rows in MXFP4, a quarter of the
+// bytes, only with tiles for three blocks (4,096 x 16,384 by 16 rows 9.5 against 10.3).
+template <int MT, int XQ, int EPI, bool NORM, typename OutT, bool X4>
 static int pick_mx4_tiles(const Mx4Args& a) {
   constexpr int ONE = EPI == MR_EPI_GATED ? 2 : 1;
+  constexpr bool MANY = X4 || XQ == 4;                    // from 9 rows on
   const int tiles = (a.n_out + 15) / 16, units = llm_compute_units();
   if (tiles <= units / 2) return launch_mx4_rows<16, MT, XQ, ONE, MT == 1 ? 2 : 1, EPI, NORM, OutT, X4>(a);
-  if (tiles <= units) return launch_mx4_rows<8, MT, XQ, ONE, STAGES, EPI, NORM, OutT, X4>(a);
-  if constexpr (MT == 1 && XQ == 4 && !X4)
-    if (tiles >= 3 * units) return launch_mx4_rows<4, MT, XQ, 2 * ONE, STAGES, EPI, NORM, OutT, X4>(a);
-  return launch_mx4_rows<4, MT, XQ, ONE, STAGES, EPI, NORM, OutT, X4>(a);
+  if (tiles <= units) return launch_mx4_rows<8, MT, XQ, ONE, MT == 1 ? 3 : 2, EPI, NORM, OutT, X4>(a);
+  if constexpr (MANY)
+    if (tiles >= 3 * units) return launch_mx4_rows<4, MT, XQ, 2 * ONE, X4 ? 2 : 1, EPI, NORM, OutT, X4>(a);
+  return launch_mx4_rows<4, MT, XQ, MANY && !X4 ? 2 * ONE : ONE, MANY ? 2 : 3, EPI, NORM, OutT, X4>(a);
 }
 
 template <int EPI, bool NORM, typename OutT, bool X4>
 static int pick_mx4_rows(const Mx4Args& a) {
   if constexpr (!X4) {
-    if (a.M <= 4) return pick_mx4_tiles<1, 1, 4, EPI, NORM, OutT, X4>(a);
-    if (a.M <= 8) return pick_mx4_tiles<1, 2, 4, EPI, NORM, OutT, X4>(a);
+    if (a.M <= 4) return pick_mx4_tiles<1, 1, EPI, NORM, OutT, X4>(a);
+    if (a.M <= 8) return pick_mx4_tiles<1, 2, EPI, NORM, OutT, X4>(a);
   }
-  if (a.M <= 16) return pick_mx4_tiles<1, 4, 4, EPI, NORM, OutT, X4>(a);
+  if (a.M <= 16) return pick_mx4_tiles<1, 4, EPI, NORM, OutT, X4>(a);
   if constexpr (!NORM) {
     // 17 to 32 rows of a weight with few tiles in two slabs of 16: blocks for twice as many units (2,048 x
     // 2,048 by 32 rows: 4.0 us against 5.4)
-    if (a.M <= 32 && (a.n_out + 15) / 16 <= llm_compute_units() / 2) return pick_mx4_tiles<1, 4, 4, EPI, NORM, OutT, X4>(a);
-    return pick_mx4_tiles<2, 4, 3, EPI, NORM, OutT, X4>(a);
+    if (a.M <= 32 && (a.n_out + 15) / 16 <= llm_compute_units() / 2) return pick_mx4_tiles<1, 4, EPI, NORM, OutT, X4>(a);
+    return pick_mx4_tiles<2, 4, EPI, NORM, OutT, X4>(a);
   }
   return LLM_ERR_ARG;
 }

@@ -90,7 +90,7 @@ class Mx4Matrix:
 class Mx4Ops:
     """The operations of ``HipOps`` on matrices in MXFP4."""
 
-    MX4_ROWS = 32           # most rows that go to the product for few rows, but for the widest weights and the smallest
+    MX4_ROWS = 32           # rows that go to the product for few rows in any case
     MX4_PLANS = 4096        # launch plans kept, by sizes
     MX4_FAR = 1 << 22       # most elements between two rows in bfloat16 for the product for many rows: a block's offsets have 32 bits
 
@@ -158,18 +158,18 @@ class Mx4Ops:
             raise KernelError("%s must be a matrix with contiguous rows" % what)
 
     # ---- products
-    def _mx4_few(self, m, n_out, four):
-        """Whether the product goes to the kernel for few rows.  Up to 16 rows always.  Up to 32 unless W
-        has tiles of outputs for three blocks a compute unit, with which the other fills the units too
-        (gate and up of 4,096 x 14,336: 32 to 35 us against 23).  Up to 64 where W has so few tiles that
-        the other would leave units idle (us, 64 rows, that kernel against this: bfloat16, K 2,048, 2,048
-        outputs 5.5 against 10.4, but K 4,096, 6,144 outputs 17.5 against 17.8 and K 14,336, 4,096
-        outputs 36 against 22; MXFP4, in the same order, 3.6 against 6.2, 8.6 against 11.1 and 18.3
-        against 17.5)."""
-        tiles = -(-n_out // TILE_ROWS)
+    def _mx4_few(self, m, n, k, four):
+        """Whether the product goes to the kernel for few rows.  Up to 32 rows always (us, 32 rows, that
+        kernel against the other: K 14,336, 4,096 outputs 19.5 against 23.0, gate and up of 4,096 x 14,336
+        22.7 against 22.8).  Up to 64, where it reads W twice, if W has at most two tiles a compute unit
+        and is small: the other cannot fill the units then (64 rows, bfloat16: K 4,096, 6,144 outputs 14.0
+        against 18.6, K 14,336, 2,048 outputs 18.2 against 22.6, but 4,096 outputs 36.1 against 24.3 and K
+        2,048, 10,240 outputs 12.9 against 11.9; MXFP4, in the same order, 9.2 against 11.0, 9.9 against
+        16.1, 20.1 against 18.8, 8.4 against 8.0).  There the wide rows of X in bfloat16 come to count (K
+        28,672, 1,024 outputs: 30.7 against 24.3)."""
         if m <= self.MX4_ROWS:
-            return m <= TILE_ROWS or tiles < 3 * self.units
-        return m <= 2 * self.MX4_ROWS and 2 * tiles <= (3 if four else 1) * self.units
+            return True
+        return m <= 2 * self.MX4_ROWS and n <= 2 * TILE_ROWS * self.units and n * k <= 1 << 25 and (four or k <= 1 << 14)
 
     # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, and the us
     # that 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much
@@ -212,7 +212,7 @@ class Mx4Ops:
         if plan is None:
             if len(self._mx4_plans) >= self.MX4_PLANS:
                 self._mx4_plans.clear()
-            few = self._mx4_few(m, n_out, four) or (k > self.MX4_FAR and not four)
+            few = self._mx4_few(m, n, k, four) or (k > self.MX4_FAR and not four)
             plan = (-1, 1) if few else self._mx4_form(m, n, k, four)
             self._mx4_plans[key] = plan
         return plan
