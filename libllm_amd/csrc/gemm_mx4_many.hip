@@ -479,7 +479,9 @@ static int launch_mx4_many(Mx4ManyArgs a) {
   const int out_tiles = (a.n_out + 15) / 16, per = EPI == MM_EPI_GATED ? BNT / 2 : BNT;
   a.m_tiles = (a.M + BM - 1) / BM;
   a.n_tiles = (out_tiles + per - 1) / per;
-  const long long blocks = 8LL * ((a.m_tiles + 7) / 8) * 8 * ((a.n_tiles + 7) / 8);   // surplus blocks leave at once
+  // Surplus blocks, where tiles of W are no multiple of 8, leave at once, but each has to be given its LDS first:
+  // none along X's rows (with bands of 8 always full, 64 rows, K 14,336 in seven slices, 4,096 outputs: 19.0 us against 16.5).
+  const long long blocks = 8LL * a.m_tiles * ((a.n_tiles + 7) / 8);
   if (blocks > 0x7fffffffLL) return LLM_ERR_ARG;
   // more than 64 KiB of LDS has to be asked for, once per device and kernel
   static bool asked[64];

@@ -166,10 +166,17 @@ class Mx4Ops:
         against 18.6, K 14,336, 2,048 outputs 18.2 against 22.6, but 4,096 outputs 36.1 against 24.3 and K
         2,048, 10,240 outputs 12.9 against 11.9; MXFP4, in the same order, 9.2 against 11.0, 9.9 against
         16.1, 20.1 against 18.8, 8.4 against 8.0).  There the wide rows of X in bfloat16 come to count (K
-        28,672, 1,024 outputs: 30.7 against 24.3)."""
+        28,672, 1,024 outputs: 30.7 against 24.3).  Beyond 64 while its blocks, a tile of W by 32 rows each,
+        are two a compute unit (MXFP4: three) and read little of X in all (K 2,048, 2,048 outputs, 128 / 192
+        rows: bfloat16 9.3 / 12.7 against 10.1 / 10.3, MXFP4 4.3 / 5.8 against 6.1 / 6.2; K 2,048, 512 outputs,
+        512 rows: 8.3 against 10.3 and 4.1 against 6.1)."""
         if m <= self.MX4_ROWS:
             return True
-        return m <= 2 * self.MX4_ROWS and n <= 2 * TILE_ROWS * self.units and n * k <= 1 << 25 and (four or k <= 1 << 14)
+        tiles = -(-n // TILE_ROWS)
+        if m <= 2 * self.MX4_ROWS:
+            return tiles <= 2 * self.units and n * k <= 1 << 25 and (four or k <= 1 << 14)
+        blocks, most = tiles * -(-m // 32), 3 if four else 2
+        return blocks <= most * self.units and blocks * k <= (3 if four else 1) << 20
 
     # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, and the us
     # that 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much
@@ -190,8 +197,8 @@ class Mx4Ops:
         best = None
         for form, rows, cols, times in self._MX4_FORMS[four]:
             blocks = -(-m // rows) * -(-n // cols)
-            for ks in (1, 2, 4, 8, 16):
-                if ks > quads or (ks > 1 and blocks * ks > 2 * self.units):
+            for ks in range(1, min(quads, 16) + 1):
+                if ks > 1 and blocks * ks > 2 * self.units:
                     break
                 per = -(-quads // ks)
                 if -(-quads // per) != ks:

@@ -755,7 +755,7 @@ class HipOps(Mx4Ops):
         if tuple(w.shape) != (n, k):
             raise KernelError("qkv_rope: the weight is %s, expected %s" % (tuple(w.shape), (n, k)))
         fused = (dtype == torch.bfloat16 and (adjacent or rot_dim == 0) and hd % 16 == 0
-                 and m <= self.SKINNY_ROWS and m == ctx.n_tokens
+                 and (m <= self.SKINNY_ROWS or isinstance(w, Mx4Matrix)) and m == ctx.n_tokens
                  and (not write or (kv is not None and "k" in kv.planes and kv.planes["k"].dtype == torch.bfloat16)))
         if isinstance(w, Mx4Matrix):
             if fused:

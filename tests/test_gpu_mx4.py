@@ -496,7 +496,7 @@ def test_added_into_the_stream(ops, m, n, k):
     xd, rd = x.double().numpy(), res.double().numpy()
     lim = bound(xd, w, k, torch.float32)
     if got is None:
-        assert m <= 2 * ops.MX4_ROWS
+        assert ops._mx4_plan(m, n, n, k, False)[0] < 0
         total = stream.double().cpu().numpy()
     else:
         assert torch.equal(stream.cpu(), res)

@@ -52,7 +52,7 @@ def test_plans_are_launches_the_kernels_take():
         assert len(ops._mx4_plans) <= 50
         assert (form, ks) == ops._mx4_plan(m, n, n // 2 if gated else n, k, four)
         if form < 0:
-            assert ks == 1 and m <= 2 * ops.MX4_ROWS
+            assert ks == 1 and (m <= 2 * ops.MX4_ROWS or -(-m // 32) * -(-n // 16) <= 3 * ops.units)
             continue
         assert form in (0, 1, 2, 3)
         quads = -(-k // 512)
