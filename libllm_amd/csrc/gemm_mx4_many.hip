@@ -406,65 +406,49 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
       }
     }
   };
-  if constexpr (sizeof(OutT) == 4) {                        // 64 bytes of a row in a store: whole pieces of lines
+  // Each wave turns its tile round through a region of LDS of its own, 16 rows of X at a time, rows 16
+  // bytes longer than they are so that the 16 rows of a write fall into different banks, and then stores
+  // whole rows: 16 bytes a lane, or where rows of C do not begin at multiples of that an element a lane,
+  // neighbours in neighbouring lanes (3,000 rows, K 64, in float32, us: 28,000 outputs 97 and straight from
+  // the sums, 64 bytes of a row at a time, 148; 28,001 outputs 118 and 249; in bfloat16 28,001 92, by eight
+  // neighbours a lane 192).
+  __syncthreads();                                          // every wave has read the last tile
+  constexpr int ES = sizeof(OutT), COLS = OUT_NT * 16, ROW_B = COLS * ES + 16, VEC = 16 / ES;
+  constexpr int LPR = COLS / VEC, RPP = 64 / LPR;           // lanes a row, rows a store
+  unsigned char* mine = lds + wave * (16 * ROW_B);
+  const bool whole = a.n_out % VEC == 0;
 #pragma unroll
-    for (int nt = 0; nt < OUT_NT; ++nt)
+  for (int mt = 0; mt < MTW; ++mt) {
 #pragma unroll
-      for (int mt = 0; mt < MTW; ++mt) {
-        const int m = m_wave + mt * 16 + r, n = n_wave + nt * 16 + 4 * g;
-        if (m >= a.M || n >= a.n_out) continue;
-        float v[4];
-        value(nt, mt, v);
-        float* dst = (float*)a.C + (size_t)m * a.n_out + n;
-        if (n + 3 < a.n_out && (a.n_out & 3) == 0) {
-          *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n + e < a.n_out) dst[e] = v[e];
-        }
-      }
-  } else {
-    // Each wave turns its tile round through a region of LDS of its own, 16 rows of X at a time, rows 16
-    // bytes longer than they are so that the 16 rows of a write fall into different banks, and then
-    // stores whole rows, 16 bytes a lane.
-    __syncthreads();                                        // every wave has read the last tile
-    constexpr int COLS = OUT_NT * 16, ROW_B = COLS * 2 + 16;
-    constexpr int LPR = COLS / 8, RPP = 64 / LPR;           // lanes a row, rows a store
-    unsigned char* mine = lds + wave * (16 * ROW_B);
-    const int col = (lane % LPR) * 8;
-#pragma unroll
-    for (int mt = 0; mt < MTW; ++mt) {
-#pragma unroll
-      for (int nt = 0; nt < OUT_NT; ++nt) {
-        float v[4];
-        value(nt, mt, v);
-        uint2 pk;
-        pk.x = pack2_bf16(v[0], v[1]);
-        pk.y = pack2_bf16(v[2], v[3]);
-        *reinterpret_cast<uint2*>(mine + r * ROW_B + (nt * 16 + 4 * g) * 2) = pk;
-      }
-      // (a wave's accesses to LDS run in order; the compiler may not move one lane's read over another's write)
-      asm volatile("" ::: "memory");
+    for (int nt = 0; nt < OUT_NT; ++nt) {
+      float v[4];
+      value(nt, mt, v);
+      unsigned char* dst = mine + r * ROW_B + (nt * 16 + 4 * g) * ES;
+      if constexpr (ES == 4) *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2_bf16(v[0], v[1]), pack2_bf16(v[2], v[3]));
+    }
+    // (a wave's accesses to LDS run in order; the compiler may not move one lane's read over another's write)
+    asm volatile("" ::: "memory");
+    const int m_tile = m_wave + mt * 16;
+    if (whole) {
+      const int n = n_wave + lane % LPR * VEC;
 #pragma unroll
       for (int pass = 0; pass < (16 + RPP - 1) / RPP; ++pass) {
         const int row = pass * RPP + lane / LPR;
-        const int m = m_wave + mt * 16 + row, n = n_wave + col;
-        if (row < 16 && m < a.M && n < a.n_out) {
-          const uint4 v = *reinterpret_cast<const uint4*>(mine + row * ROW_B + col * 2);
-          bf16_t* dst = (bf16_t*)a.C + (size_t)m * a.n_out + n;
-          if (n + 7 < a.n_out && (a.n_out & 7) == 0) {
-            *reinterpret_cast<uint4*>(dst) = v;
-          } else {
-            const uint32_t w4[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < a.n_out) dst[e] = (bf16_t)(w4[e >> 1] >> (16 * (e & 1)));
-          }
-        }
+        if (row < 16 && m_tile + row < a.M && n < a.n_out)
+          *reinterpret_cast<uint4*>((OutT*)a.C + (size_t)(m_tile + row) * a.n_out + n) =
+              *reinterpret_cast<const uint4*>(mine + row * ROW_B + lane % LPR * 16);
       }
-      asm volatile("" ::: "memory");
+    } else {
+      const int n = n_wave + lane % COLS;
+#pragma unroll
+      for (int row0 = 0; row0 < 16; row0 += 64 / COLS) {
+        const int row = row0 + lane / COLS;
+        if (m_tile + row < a.M && n < a.n_out)
+          ((OutT*)a.C)[(size_t)(m_tile + row) * a.n_out + n] = reinterpret_cast<const OutT*>(mine + row * ROW_B)[lane % COLS];
+      }
     }
+    asm volatile("" ::: "memory");
   }
 }
 
@@ -473,7 +457,7 @@ static int launch_mx4_many(Mx4ManyArgs a) {
   typedef ManyShape<X4, NBUF, EARLY, WM, WN, MTW, NTW> Shape;
   constexpr int BM = Shape::BM, BNT = Shape::BNT, NW = WM * WN;
   constexpr int OUT_NT = EPI == MM_EPI_GATED ? NTW / 2 : NTW;
-  constexpr int TURN = NW * 16 * (OUT_NT * 32 + 16);
+  constexpr int TURN = NW * 16 * (OUT_NT * 16 * (int)sizeof(OutT) + 16);
   constexpr int LDS_BYTES = Shape::BYTES > TURN ? Shape::BYTES : TURN;
   static_assert(LDS_BYTES <= 160 * 1024, "shared memory of a unit");
   const int out_tiles = (a.n_out + 15) / 16, per = EPI == MM_EPI_GATED ? BNT / 2 : BNT;

@@ -178,16 +178,16 @@ class Mx4Ops:
         blocks, most = tiles * -(-m // 32), 3 if four else 2
         return blocks <= most * self.units and blocks * k <= (3 if four else 1) << 20
 
-    # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, and the us
-    # that 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much
-    # again for every four).  Measured over 2,048 to 14,336 elements of K, 33 to 4,096 rows, 2,048 to
-    # 28,672 outputs; the forms' times cross where this says within a tenth.
+    # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, the us that
+    # 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much again for
+    # every four), and as how many such elements more a block's begin and end count.  Fitted to 90 products
+    # of each kind, 128 to 14,336 elements of K, 64 to 4,096 rows, 2,048 to 28,672 outputs, in every form:
+    # what this says is best takes 0.1 % longer than the best on average, 6 % at most (MXFP4 0.3 and 12).
     _MX4_FORMS = {
-        False: ((0, 256, 256, (2.7, 5.4, 8.1, 10.8)), (1, 128, 256, (1.45, 2.8, 4.2, 5.6)),
-                (2, 64, 128, (0.71, 1.0, 1.43, 1.75)),
-                (3, 64, 128, (0.58, 1.15, 1.75, 2.3))),
-        True: ((0, 256, 256, (0.94, 1.88, 2.82, 3.76)), (1, 128, 128, (0.49, 0.63, 1.14, 1.33)),
-               (2, 64, 128, (0.38, 0.44, 0.72, 0.85)), (3, 64, 128, (0.26, 0.52, 0.78, 1.04))),
+        False: ((0, 256, 256, (2.44, 4.87, 7.31, 9.74), 5), (1, 128, 256, (1.24, 2.49, 3.73, 4.98), 5),
+                (2, 64, 128, (0.85, 1.03, 1.38, 1.67), 0.5), (3, 64, 128, (0.64, 1.28, 1.92, 2.56), 1)),
+        True: ((0, 256, 256, (0.94, 1.88, 2.82, 3.76), 0), (1, 128, 128, (0.49, 0.63, 1.14, 1.33), 0),
+               (2, 64, 128, (0.38, 0.44, 0.72, 0.85), 0), (3, 64, 128, (0.26, 0.52, 0.78, 1.04), 0)),
     }
 
     def _mx4_form(self, m, n, k, four):
@@ -195,7 +195,7 @@ class Mx4Ops:
         adding of the slices (each written and read in 32 bits, and a launch) come out lowest."""
         quads, all_units = -(-k // QUAD), -(-k // 128)
         best = None
-        for form, rows, cols, times in self._MX4_FORMS[four]:
+        for form, rows, cols, times, more in self._MX4_FORMS[four]:
             blocks = -(-m // rows) * -(-n // cols)
             for ks in range(1, min(quads, 16) + 1):
                 if ks > 1 and blocks * ks > 2 * self.units:
@@ -204,7 +204,7 @@ class Mx4Ops:
                 if -(-quads // per) != ks:
                     continue
                 a_unit = -(-blocks * ks // self.units)
-                cost = min(4 * per, all_units) * (times[3] * ((a_unit - 1) // 4) + times[(a_unit - 1) % 4])
+                cost = (min(4 * per, all_units) + more) * (times[3] * ((a_unit - 1) // 4) + times[(a_unit - 1) % 4])
                 if ks > 1:
                     cost += 5.0 + ks * m * n * 8 / 3e6
                 if best is None or cost < best[0]:
