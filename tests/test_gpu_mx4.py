@@ -179,6 +179,30 @@ def test_quantize_rows_that_lie_apart(ops):
         assert torch.equal(q.codes, c.codes) and torch.equal(q.scales, c.scales)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("ld", [304, 300, 302, 301])
+def test_quantize_ends_of_rows(ops, ld, dtype):
+    """Rows that begin at every alignment and end anywhere in a piece of 8, numbers behind them: as if alone."""
+    big = normal((19, ld), ld, dtype=dtype).cuda()
+    for k in (1, 7, 8, 9, 127, 132, 187, 260):
+        codes, scales = quantise(big[:, :k].double().cpu().numpy())
+        got = rows_of(ops.quantize_mx4(big[:, :k]))
+        assert np.array_equal(got[0][:19, :k], codes) and not got[0][:, k:].any()
+        assert np.array_equal(got[1][:19, :scales.shape[1]], scales) and not got[1][:, scales.shape[1]:].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_reading_back_more_than_the_caches_hold(ops, dtype):
+    rows, width = (12304, 4112) if dtype == torch.float32 else (24600, 4104)
+    q = ops.quantize_mx4(torch.randn((rows, width), generator=torch.Generator(device="cuda").manual_seed(6), device="cuda"))
+    got = ops.dequantize_mx4(q, dtype)
+    assert got.numel() * got.element_size() >= 192 << 20
+    part = ops.dequantize_mx4(q.leading_rows(12288), dtype)
+    assert torch.equal(got[:12288], part)
+    again = ops.quantize_mx4(got)
+    assert torch.equal(q.codes, again.codes) and torch.equal(q.scales, again.scales)
+
+
 @pytest.mark.parametrize("n,k", [(1, 1), (16, 32), (33, 63), (18, 160), (50, 1001)])
 def test_from_codes(ops, n, k):
     rng = np.random.default_rng(n + k)
