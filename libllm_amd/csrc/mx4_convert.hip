@@ -23,13 +23,19 @@
 template <typename T>
 __device__ __forceinline__ void stage_rows(const T* X, size_t ldx, int M, int K, int row0, int u, int lane, float* mine) {
   const int k = u * MX4_UNIT + lane;
+  const int ka = min(k, K - 1), kb = min(k + 64, K - 1);       // (no load hangs on a condition: all of them go out at once)
+  T a[16], b[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const T* p = X + (size_t)min(row0 + i, M - 1) * ldx;
+    a[i] = p[ka];
+    b[i] = p[kb];
+  }
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const bool on = row0 + i < M;
-    const T* p = X + (size_t)(row0 + i) * ldx + k;
-    const float a = on && k < K ? Conv<T>::load(p) : 0.f, b = on && k + 64 < K ? Conv<T>::load(p + 64) : 0.f;
-    mine[i * CV_LD + lane] = a;
-    mine[i * CV_LD + lane + 64] = b;
+    mine[i * CV_LD + lane] = on && k < K ? Conv<T>::load(&a[i]) : 0.f;
+    mine[i * CV_LD + lane + 64] = on && k + 64 < K ? Conv<T>::load(&b[i]) : 0.f;
   }
 }
 
