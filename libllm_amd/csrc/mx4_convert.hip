@@ -234,9 +234,23 @@ __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* __restrict
 // products, which read 16 bytes at a time, where K or the address is no multiple of that.
 __global__ __launch_bounds__(256) void pad_rows_kernel(const bf16_t* __restrict__ X, size_t ldx,
                                                        bf16_t* __restrict__ out, int M, int K, int ldo) {
-  for (size_t m = blockIdx.x; m < (size_t)M; m += gridDim.x)
-    for (int k = blockIdx.y * 256 + threadIdx.x; k < ldo; k += gridDim.y * 256)
-      out[m * ldo + k] = k < K ? X[m * ldx + k] : (bf16_t)0;
+  // (two neighbours a thread and store, eight loads at once; ldo is even)
+  for (size_t m = blockIdx.x; m < (size_t)M; m += gridDim.x) {
+    const bf16_t* x = X + m * ldx;
+    for (int k0 = (blockIdx.y * 1024 + threadIdx.x) * 2; k0 < ldo; k0 += gridDim.y * 2048) {
+      uint32_t lo[4], hi[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        lo[i] = x[min(k0 + i * 512, K - 1)];
+        hi[i] = x[min(k0 + i * 512 + 1, K - 1)];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int k = k0 + i * 512;
+        if (k < ldo) *reinterpret_cast<uint32_t*>(out + m * ldo + k) = (k < K ? lo[i] : 0) | (k + 1 < K ? hi[i] << 16 : 0);
+      }
+    }
+  }
 }
 
 static inline dim3 mx4_grid(int rows, int k) { return dim3(mx4_tiles(rows), mx4_quads(k)); }
@@ -300,7 +314,7 @@ extern "C" int llm_mx4_pack(const void* rows, size_t ldc, const void* row_scales
 
 extern "C" int llm_pad_rows(const void* X, size_t ldx, void* out, int M, int K, int ldo, hipStream_t stream) {
   if (M <= 0) return LLM_OK;
-  if (K <= 0 || ldx < (size_t)K || ldo < K || X == nullptr || out == nullptr) return LLM_ERR_ARG;
+  if (K <= 0 || ldx < (size_t)K || ldo < K || (ldo & 1) || X == nullptr || out == nullptr || (((uintptr_t)out) & 3)) return LLM_ERR_ARG;
   const dim3 grid(M < (1 << 16) ? M : 1 << 16, ldo < (1 << 19) ? (ldo + 2047) / 2048 : 256);
   pad_rows_kernel<<<grid, 256, 0, stream>>>((const bf16_t*)X, ldx, (bf16_t*)out, M, K, ldo);
   return llm_launch_status();
