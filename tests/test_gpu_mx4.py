@@ -709,3 +709,73 @@ def test_generation_and_the_other_entry_points(models, tmp_path):
         Model(path, dtype="float32", weights="mxfp4")
     with pytest.raises(ConfigError):
         Model(path, weights="int4")
+
+
+@pytest.mark.parametrize("program", ["python", "native"])
+def test_command_lines(models, program):
+    import os
+    import subprocess
+    import sys
+
+    from libllm_amd import Model
+    from libllm_amd.hip import build
+    path = models["B"][0]
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    command = {"python": [sys.executable, os.path.join(root, "bin", "llm")],
+               "native": [os.path.join(os.path.dirname(build.build_capi(force=False, verbose=False)), build.CLI_NAME)]}[program]
+    command += ["chat", "-m", path, "-ids", "-temperature", "0", "-max_new_tokens", "6"]
+    run = lambda *flags: subprocess.run(command + list(flags), input="11 12 13 14\n", capture_output=True, text=True, timeout=120)
+    got = run("-weights", "mxfp4")
+    assert got.returncode == 0, got.stderr
+    reply = [l for l in got.stdout.splitlines() if l.startswith("> ") and len(l) > 2][0][2:].split()
+    model = Model(path, max_tokens=1024, weights="mxfp4")
+    want = model.generate([[11, 12, 13, 14]], max_new_tokens=6, temperature=0.0)[0]
+    assert [int(t) for t in reply] == [t for t in want if not model.is_stop(t)]
+    assert run("-weights", "int4").returncode == 2
+    got = run("-weights", "mxfp4", "-dtype", "float32")
+    assert got.returncode != 0 and "bfloat16" in got.stderr
+
+
+def test_time_per_operation(models):
+    """Timed, the operations give what they give otherwise, the quantiser among them."""
+    from libllm_amd import Model
+    from libllm_amd.hip import HipOps
+    path, prompts = models["B"][0], [[5, 6, 7, 8, 9], [11, 12]]
+    plain = Model(path, max_tokens=512, weights="mxfp4").generate(prompts, max_new_tokens=6, temperature=0.0, stop_tokens=())
+    ops = HipOps()
+    ops.start_timing()
+    timed = Model(path, max_tokens=512, weights="mxfp4", ops=ops)
+    assert timed.generate(prompts, max_new_tokens=6, temperature=0.0, stop_tokens=()) == plain
+    report = dict((name, (calls, ms)) for name, calls, ms in ops.timing_report())
+    assert report["quantize_mx4"][0] >= 4 and all(ms > 0 for _, ms in report.values())
+
+
+def test_from_two_threads(ops):
+    """Two host threads with a stream each, products of many sizes at once: each as it is alone."""
+    import threading
+    w = ops.quantize_mx4(normal((96, 640), 1, 0.1).cuda())
+    rows = [normal((m, 640), m, dtype=torch.bfloat16).cuda() for m in (1, 5, 16, 20, 40, 70, 130, 300)]
+    work = lambda x: [ops.linear(x, w, None, torch.float32), ops.linear(ops.quantize_mx4(x), w, None, torch.bfloat16),
+                      ops.linear_swiglu(x, w)]
+    want = [work(x) for x in rows]
+    torch.cuda.synchronize()
+    got, failed = {}, []
+
+    def run(name):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(20):
+                    got[name] = [work(x) for x in rows]
+            stream.synchronize()
+        except Exception as e:                              # (a thread's exception would be lost)
+            failed.append(e)
+    threads = [threading.Thread(target=run, args=(name,)) for name in "ab"]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
+    for name in "ab":
+        for a, b in zip(want, got[name]):
+            assert all(torch.equal(p, q) for p, q in zip(a, b))
