@@ -55,11 +55,11 @@ class Mx4Matrix:
         self.codes_ptr, self.scales_ptr = codes.data_ptr(), scales.data_ptr()
 
     @classmethod
-    def _new(cls, rows, width, device):
+    def _new(cls, rows, width, device, blank):
         """Room for a matrix: one allocation, the codes first."""
         q = cls.__new__(cls)
         cells = -(-rows // TILE_ROWS) * -(-width // QUAD)
-        q._storage = both = torch.empty(cells * 4352, dtype=torch.uint8, device=device)
+        q._storage = both = blank.new_empty(cells * 4352)
         q.shape, q.device, q.codes_ptr = (rows, width), device, both.data_ptr()
         q.scales_ptr = q.codes_ptr + cells * 4096
         return q
@@ -100,12 +100,12 @@ class Mx4Ops:
             raise KernelError("an MXFP4 matrix has rows and columns, not [%d, %d]" % (rows, width))
         if rows > 1 << 27 or width > 65535 * QUAD:          # (threads of a launch, blocks along the second axis of a grid)
             raise KernelError("an MXFP4 matrix of [%d, %d] is too large" % (rows, width))
-        return Mx4Matrix._new(rows, width, self.device)
+        return Mx4Matrix._new(rows, width, self.device, self._blank[torch.uint8])
 
     def _mx4(self, q, what):
         if not isinstance(q, Mx4Matrix):
             raise KernelError("%s is no MXFP4 matrix" % what)
-        if q.device != self.device:
+        if q.device is not self.device and q.device != self.device:
             raise KernelError("%s lies on %s, not on %s" % (what, q.device, self.device))
         return q
 
@@ -126,7 +126,7 @@ class Mx4Ops:
         self._mx4(q, "the matrix to read")
         code = self._dtype_code(dtype)
         m, k = q.shape
-        out = torch.empty((m, k), dtype=dtype, device=self.device)
+        out = self._blank[dtype].new_empty(m, k)
         self._launch("llm_mx4_dequantize", q.codes_ptr, q.scales_ptr, out.data_ptr(), code, m, k)
         return out
 
@@ -150,7 +150,7 @@ class Mx4Ops:
 
     def _matrix(self, x, what):
         """A matrix on the device with contiguous rows."""
-        if x.dim() == 2 and x.is_contiguous() and x.device == self.device:
+        if x.is_contiguous() and x.get_device() == self._index and x.dim() == 2:
             return
         if x.device != self.device:
             raise KernelError("%s lies on %s, not on %s" % (what, x.device, self.device))
@@ -229,8 +229,6 @@ class Mx4Ops:
         padded copy where its length, distance or address does not allow that; with its address and
         the distance of its rows."""
         at = x.data_ptr()
-        if x.dtype is torch.bfloat16 and k % piece == 0 and at % 16 == 0 and x.is_contiguous() and x.device == self.device:
-            return x, at, k
         if x.dtype != torch.bfloat16:
             raise KernelError("linear: an MXFP4 weight takes rows in bfloat16 or MXFP4, not %s" % (x.dtype,))
         self._matrix(x, "linear input")
@@ -246,7 +244,8 @@ class Mx4Ops:
         """The product of ``x`` (a matrix, MXFP4 rows, or a record of normed rows whose norm is
         prepared) with ``w``.  ``stack``: where K goes in slices their products may come back
         unadded, ``[slices, m, n]`` in 32 bits."""
-        self._mx4(w, "the weight")
+        if w.device is not self.device:
+            self._mx4(w, "the weight")
         n, k = w.shape
         four, ssq, eps = False, None, 0.0
         if not isinstance(x, torch.Tensor):
@@ -261,18 +260,20 @@ class Mx4Ops:
         code = self._dtype_code(out_dtype)
         bptr = None if bias is None else self._dev(bias, "bias", torch.float32, (n,))
         if m == 0:
-            return torch.empty((m, n_out), dtype=out_dtype, device=self.device)
+            return self._blank[out_dtype].new_empty(m, n_out)
         form, ks = self._mx4_plans.get((m, n, n_out, k, four)) or self._mx4_plan(m, n, n_out, k, four)
         piece = 8 if form < 0 else 128
         if four:
             xp, xs, ldx = x.codes_ptr, x.scales_ptr, 0
         else:
-            x, xp, ldx = self._mx4_rows(x, k, piece)
-            xs = None
+            xp, xs, ldx = x.data_ptr(), None, k
+            if not (x.dtype is torch.bfloat16 and k % piece == 0 and xp % 16 == 0 and x.is_contiguous()
+                    and x.get_device() == self._index):
+                x, xp, ldx = self._mx4_rows(x, k, piece)
         kp = -(-k // piece) * piece         # (where rows were padded, their length: the weight's codes there are zero)
         wp, ws = w.codes_ptr, w.scales_ptr
         if ks == 1:
-            out = torch.empty((m, n_out), dtype=out_dtype, device=self.device)
+            out = self._blank[out_dtype].new_empty(m, n_out)
             if form < 0:
                 self._launch("llm_gemm_mx4_rows", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp,
                              None, None, None, ssq, eps)
@@ -280,17 +281,17 @@ class Mx4Ops:
                 self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, bptr, out.data_ptr(), epilogue, code, m, n, kp,
                              form, 1)
             return out
-        parts = torch.empty((ks, m, n), dtype=torch.float32, device=self.device)
+        parts = self._blank[torch.float32].new_empty(ks, m, n)
         self._launch("llm_gemm_mx4_many", xp, xs, ldx, wp, ws, None, parts.data_ptr(), self._EPI_NONE,
                      self._dtype_code(torch.float32), m, n, kp, form, ks)
         if stack and bias is None and epilogue == self._EPI_NONE:
             return parts
-        out = torch.empty((m, n_out), dtype=out_dtype, device=self.device)
+        out = self._blank[out_dtype].new_empty(m, n_out)
         self._launch("llm_mx4_join", parts.data_ptr(), ks, bptr, out.data_ptr(), epilogue, code, m, n)
         return out
 
     def _mx4_input(self, x, w):
-        """``x`` for a product with ``w``: a record of normed rows goes in as it is where the product before
+        """``x`` for a product with ``w``: a matrix as it is; a record of normed rows goes in as it is where the product before
         has prepared its norm and the product for few rows takes it, else the norm kernel runs."""
         if isinstance(x, (torch.Tensor, Mx4Matrix)):
             return x
@@ -301,7 +302,8 @@ class Mx4Ops:
     def _linear_mx4(self, x, w, bias, out_dtype, residual=None, then_norm=None):
         """``linear`` with an MXFP4 weight.  With ``residual`` the product for few rows adds into it;
         the other returns the product, or its slices of K, for the norm that comes next to add."""
-        x = self._mx4_input(x, w)
+        if not isinstance(x, torch.Tensor):
+            x = self._mx4_input(x, w)
         n, k = w.shape
         if residual is None or bias is not None or not isinstance(x, torch.Tensor):
             return self._mx4_product(x, w, n, out_dtype, self._EPI_NONE, bias, residual is not None)

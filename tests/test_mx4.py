@@ -30,7 +30,7 @@ def test_matrix_checks_its_storage():
                 ((20, 100), torch.zeros(8193, dtype=torch.uint8)[1:], scales)):
         with pytest.raises(KernelError):
             Mx4Matrix(*bad)
-    room = Mx4Matrix._new(20, 100, "cpu")
+    room = Mx4Matrix._new(20, 100, codes.device, codes[:0])
     assert room.codes.shape == (8192,) and room.scales.shape == (512,)
     assert room.codes_ptr == room.codes.data_ptr() and room.scales_ptr == room.scales.data_ptr()
 
