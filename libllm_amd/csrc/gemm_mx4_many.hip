@@ -488,11 +488,13 @@ static int launch_mx4_many(Mx4ManyArgs a) {
 // 167).  2, 64 x 128: several blocks a unit, which cover each other's waits.  3, 64 x 128 with four tiles of
 // K held and fragments two steps ahead: for a block a unit or less, where a block waits for memory (1.5 us
 // from a weight that no cache holds).  In bfloat16 that form has eight waves (128 rows, K 4,096, 6,144
-// outputs, us: 19.6, by four waves 22.3, form 2 22.9).
+// outputs, us: 19.6, by four waves 22.3, form 2 22.9).  4, 64 x 64, for products that even so give a block to a
+// fraction of the units (128 rows, us by form 3 and 4: K 2,048, 2,048 outputs in bfloat16 10.8 and 9.5, in MXFP4 6.6
+// and 5.8, K 4,096, 6,144 outputs in MXFP4 10.1 and 8.2); in MXFP4 it holds six tiles of K (four: 8.8).
 // Left as they are, measured: four tiles of 128 elements instead of two of 256 in form 0 of MXFP4 (61.2 us
 // against 59.6 at 4,096 rows, K 4,096, 6,144 outputs), and the widening taken out of form 0 in bfloat16
 // (no change): neither latency nor the vector units bound the large products.
-#define MM_FORMS 4
+#define MM_FORMS 5
 template <bool X4, int EPI, typename OutT>
 static int pick_mx4_many(const Mx4ManyArgs& a, int form) {
   if constexpr (X4) {
@@ -501,6 +503,7 @@ static int pick_mx4_many(const Mx4ManyArgs& a, int form) {
       case 1: return launch_mx4_many<true, 2, false, 2, 2, 4, 4, EPI, OutT>(a);
       case 2: return launch_mx4_many<true, 2, false, 1, 4, 4, 2, EPI, OutT>(a);
       case 3: return launch_mx4_many<true, 4, true, 1, 4, 4, 2, EPI, OutT>(a);
+      case 4: return launch_mx4_many<true, 6, true, 2, 2, 2, 2, EPI, OutT>(a);
     }
   } else {
     switch (form) {
@@ -508,6 +511,7 @@ static int pick_mx4_many(const Mx4ManyArgs& a, int form) {
       case 1: return launch_mx4_many<false, 3, false, 2, 4, 4, 4, EPI, OutT>(a);
       case 2: return launch_mx4_many<false, 2, false, 1, 4, 4, 2, EPI, OutT>(a);
       case 3: return launch_mx4_many<false, 4, true, 2, 4, 2, 2, EPI, OutT>(a);
+      case 4: return launch_mx4_many<false, 4, true, 2, 2, 2, 2, EPI, OutT>(a);
     }
   }
   return LLM_ERR_ARG;
@@ -524,7 +528,7 @@ static int mx4_many(const Mx4ManyArgs& a, int epilogue, int out_dtype, int form)
 // W [N, K] as mx4.h lays it out.  X: bfloat16 rows ldx apart with xs null (their length K and ldx
 // multiples of 128, what lies beyond W's width zero), or codes with their scales in xs.  epilogue 0:
 // C [M, N] of out_dtype, plus bias[n] if not null; 1 | act << 4: C [M, N / 2] in bfloat16, the gate
-// through an activation of common.h, N / 2 a multiple of 16.  form: 0 .. 3, see above.  With k_split
+// through an activation of common.h, N / 2 a multiple of 16.  form: 0 .. 4, see above.  With k_split
 // above 1 (epilogue 0, float32, no bias) C is [k_split, M, N], the products over as many slices of K of
 // ceil(quads / k_split) quads of 512 elements; every slice has elements.
 extern "C" int llm_gemm_mx4_many(const void* X, const void* xs, int ldx, const void* wc, const void* ws,

@@ -161,33 +161,35 @@ class Mx4Ops:
     def _mx4_few(self, m, n, k, four):
         """Whether the product goes to the kernel for few rows.  Up to 32 rows always (us, 32 rows, that
         kernel against the other: K 14,336, 4,096 outputs 19.5 against 23.0, gate and up of 4,096 x 14,336
-        22.7 against 22.8).  Up to 64, where it reads W twice, if W has at most two tiles a compute unit
-        and is small: the other cannot fill the units then (64 rows, bfloat16: K 4,096, 6,144 outputs 14.0
-        against 18.6, K 14,336, 2,048 outputs 18.2 against 22.6, but 4,096 outputs 36.1 against 24.3 and K
-        2,048, 10,240 outputs 12.9 against 11.9; MXFP4, in the same order, 9.2 against 11.0, 9.9 against
-        16.1, 20.1 against 18.8, 8.4 against 8.0).  There the wide rows of X in bfloat16 come to count (K
-        28,672, 1,024 outputs: 30.7 against 24.3).  Beyond 64 while its blocks, a tile of W by 32 rows each,
-        are two a compute unit (MXFP4: three) and read little of X in all (K 2,048, 2,048 outputs, 128 / 192
-        rows: bfloat16 9.3 / 12.7 against 10.1 / 10.3, MXFP4 4.3 / 5.8 against 6.1 / 6.2; K 2,048, 512 outputs,
-        512 rows: 8.3 against 10.3 and 4.1 against 6.1)."""
+        22.7 against 22.8).  Up to 64, where it reads W twice, if W is small and has two tiles a compute
+        unit at most (MXFP4: one and a half), so that the other cannot fill the units (64 rows, bfloat16:
+        K 2,048, 6,144 outputs 8.9 against 10.4, K 8,192, 2,048 outputs 12.3 against 13.4, but K 2,048, 10,240
+        outputs 12.9 against 10.8, K 14,336, 2,048 outputs 18.2 against 16.6; MXFP4, in the same order, 6.1
+        against 6.5, 7.0 against 10.6, 8.4 against 6.8, 9.8 against 12.6: wide rows count for less there).
+        Beyond 64 while its blocks, a tile of W by 32 rows each, are two a compute unit (MXFP4: two and a
+        half) and read little of X in all (K 2,048, 2,048 outputs, 128 / 192 rows: bfloat16 9.3 / 12.7 against
+        9.5 / 9.6, MXFP4 4.3 / 5.8 against 5.7 / 5.8; K 2,048, 512 outputs, 512 rows: 8.3 against 10.3 and
+        4.1 against 6.1)."""
         if m <= self.MX4_ROWS:
             return True
         tiles = -(-n // TILE_ROWS)
         if m <= 2 * self.MX4_ROWS:
-            return tiles <= 2 * self.units and n * k <= 1 << 25 and (four or k <= 1 << 14)
-        blocks, most = tiles * -(-m // 32), 3 if four else 2
-        return blocks <= most * self.units and blocks * k <= (3 if four else 1) << 20
+            return 2 * tiles <= (3 if four else 4) * self.units and n * k <= 1 << 25 and k <= 1 << (14 if four else 13)
+        blocks = tiles * -(-m // 32)
+        return 2 * blocks <= (5 if four else 4) * self.units and blocks * k <= (2 if four else 1) << 20
 
     # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, the us that
     # 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much again for
-    # every four), and as how many such elements more a block's begin and end count.  Fitted to 90 products
-    # of each kind, 128 to 14,336 elements of K, 64 to 4,096 rows, 2,048 to 28,672 outputs, in every form:
-    # what this says is best takes 0.1 % longer than the best on average, 6 % at most (MXFP4 0.3 and 12).
+    # every four), and as how many such elements more a block's begin and end count.  Fitted to 135
+    # products of each kind, 128 to 14,336 elements of K, 64 to 4,096 rows, 2,048 to 28,672 outputs, in every
+    # form: what this says is best takes 0.1 % longer than the best on average, 4 % at most.
     _MX4_FORMS = {
-        False: ((0, 256, 256, (2.44, 4.87, 7.31, 9.74), 5), (1, 128, 256, (1.24, 2.49, 3.73, 4.98), 5),
-                (2, 64, 128, (0.85, 1.03, 1.38, 1.67), 0.5), (3, 64, 128, (0.64, 1.28, 1.92, 2.56), 1)),
-        True: ((0, 256, 256, (0.94, 1.88, 2.82, 3.76), 0), (1, 128, 128, (0.49, 0.63, 1.14, 1.33), 0),
-               (2, 64, 128, (0.38, 0.44, 0.72, 0.85), 0), (3, 64, 128, (0.26, 0.52, 0.78, 1.04), 0)),
+        False: ((0, 256, 256, (2.56, 5.12, 7.68, 10.24), 1.5), (1, 128, 256, (1.255, 2.51, 3.765, 5.02), 4.5),
+                (2, 64, 128, (0.69, 0.92, 1.07, 1.75), 0), (3, 64, 128, (0.58, 1.15, 1.73, 2.31), 0.5),
+                (4, 64, 64, (0.58, 1.17, 1.75, 2.34), 0)),
+        True: ((0, 256, 256, (0.83, 1.66, 2.48, 3.31), 0), (1, 128, 128, (0.265, 0.36, 1.26, 1.34), 0),
+               (2, 64, 128, (0.25, 0.26, 0.51, 1.13), 0), (3, 64, 128, (0.21, 0.42, 0.63, 0.84), 1),
+               (4, 64, 64, (0.17, 0.34, 0.51, 0.68), 0)),
     }
 
     def _mx4_form(self, m, n, k, four):

@@ -300,7 +300,7 @@ def test_gated(ops, m, inter, k, four, act):
     assert (np.abs(got.double().cpu().numpy() - want) <= lim).all()
 
 
-FORMS = {False: (0, 1, 2, 3), True: (0, 1, 2, 3)}
+FORMS = {False: (0, 1, 2, 3, 4), True: (0, 1, 2, 3, 4)}
 
 
 @pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
