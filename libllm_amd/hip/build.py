@@ -99,11 +99,8 @@ def _lib_dirs() -> List[str]:
 def _writable(d: str) -> bool:
     try:
         os.makedirs(d, exist_ok=True)
-        probe = os.path.join(d, ".probe-%d" % os.getpid())
-        with open(probe, "w"):
-            pass
-        os.remove(probe)
-        return True
+        with tempfile.TemporaryFile(dir=d):             # (a name of its own: threads of one process may look at once)
+            return True
     except OSError:
         return False
 

@@ -96,3 +96,11 @@ def test_two_processes_that_find_nothing_built_build_once(tmp_path, monkeypatch)
         t.join()
     assert got == [os.path.join(target, build.LIB_NAME)] * 2 and len(calls) == 1
     assert build.build(force=False, verbose=False) == got[0] and len(calls) == 1      # and it stays built
+
+
+def test_a_folder_is_writable_to_many_threads_at_once(tmp_path):
+    from concurrent.futures import ThreadPoolExecutor
+    from libllm_amd.hip import build
+    with ThreadPoolExecutor(max_workers=8) as pool:
+        assert all(pool.map(lambda _: build._writable(str(tmp_path / "lib")), range(400)))
+    assert os.listdir(tmp_path / "lib") == []
