@@ -9,15 +9,15 @@
 // 16 WN NTW rows of W (gated: half of them gate, half the up rows of the same columns); W is the A
 // operand, so that a lane ends with four consecutive columns of one row of C.  K goes by in tiles:
 // 128 elements (bfloat16, four steps of 32) or 256 (MXFP4, two steps of 128).  X's tiles go from
-// memory straight into LDS (global_load_lds_dwordx4), two buffers.  In bfloat16 a row of a tile is 256
-// bytes in 16 pieces; piece p of row r lies at p ^ (r & 15), so that the 16 rows a fragment read
-// touches fall into different banks.  In MXFP4 the tiles lie in lane order as they come.  W's codes
-// are a quarter of X's bytes: with rows in bfloat16 they stay in registers, read straight from the
-// caches by every wave that needs them, one tile of K ahead; with rows in MXFP4 they go through LDS
-// like X's, and the scales too, four units at a time.
+// memory straight into LDS (global_load_lds_dwordx4), two to six buffers by form.  In bfloat16 a row of
+// a tile is 256 bytes in 16 pieces; piece p of row r lies at p ^ (r & 15), so that the 16 rows a fragment
+// read touches fall into different banks.  In MXFP4 the tiles lie in lane order as they come.  W's codes
+// are a quarter of X's bytes: with rows in bfloat16 and two buffers they stay in registers, read straight
+// from the caches by every wave that needs them, one tile of K ahead; with more buffers, and with rows in
+// MXFP4, they go through LDS like X's, and the scales too, four units at a time.
 //
-// The fragments of a step are read into registers one step ahead of the matrix instructions that use
-// them, dealt out between those; the barrier of a tile lies in front of its last step, whose
+// The fragments of a step are read into registers one step (EARLY: two) ahead of the matrix instructions
+// that use them, dealt out between those; the barrier of a tile lies in front of its last step, whose
 // fragments every wave has by then: behind it the loads of a later tile go out into the buffer that
 // is left, and the first fragments of the next tile are read.
 #include "mx4.h"
