@@ -23,7 +23,7 @@ typedef uint16_t bf16_t;     // bfloat16 as raw bits: the upper half of an IEEE 
 __device__ __forceinline__ float llm_gated(int act, float g, float u) {
   if (act == LLM_ACT_GELU_TANH)
     return u * (0.5f * g * (1.0f + tanhf(0.7978845608028654f * (g + 0.044715f * g * g * g))));
-  if (act == LLM_ACT_RELU) return g > 0.f ? u * g : 0.f;
+  if (act == LLM_ACT_RELU) return u * (g < 0.f ? 0.f : g);        // (NaN, of either, stays)
   return u * g / (1.0f + expf(-g));
 }
 
