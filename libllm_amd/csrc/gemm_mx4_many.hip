@@ -398,9 +398,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_mx4_many_kernel(Mx4ManyArgs
     for (int e = 0; e < 4; ++e) {
       v[e] = acc[nt][mt][e];
       if (GATED) {
-        const float gt = acc[nt][mt][e], up = acc[nt + NTW / 2 < NTW ? nt + NTW / 2 : nt][mt][e];
-        v[e] = a.act == LLM_ACT_SILU ? up * (gt * __builtin_amdgcn_rcpf(1.0f + fast_exp2(-1.4426950408889634f * gt)))
-                                     : llm_gated(a.act, gt, up);      // (the order: mx4_gated)
+        v[e] = mx4_gated<sizeof(OutT) == 4>(a.act, acc[nt][mt][e], acc[nt + NTW / 2 < NTW ? nt + NTW / 2 : nt][mt][e]);
       } else {
         v[e] += bias[nt][e];
       }
@@ -596,7 +594,7 @@ __global__ __launch_bounds__(256) void mx4_join_kernel(const float* __restrict__
   }
 #pragma unroll
   for (int e = 0; e < VEC; ++e) {
-    if (GATED) v[e] = mx4_gated(act, v[e], u[e]);
+    if (GATED) v[e] = mx4_gated<sizeof(OutT) == 4>(act, v[e], u[e]);
     else if (bias != nullptr) v[e] += bias[n + e];
   }
   OutT* dst = C + m * n_out + n;

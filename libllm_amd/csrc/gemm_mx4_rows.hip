@@ -267,7 +267,7 @@ __global__ __launch_bounds__(WAVES * 64) void gemm_mx4_rows_kernel(Mx4Args a) {
       if (on) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if (EPI == MR_EPI_GATED) v[0][e] = mx4_gated(a.act, v[0][e], v[RPR - 1][e]);
+          if (EPI == MR_EPI_GATED) v[0][e] = mx4_gated<sizeof(OutT) == 4>(a.act, v[0][e], v[RPR - 1][e]);
           else if (EPI == MR_EPI_ACCUM) v[0][e] += e_prev[ort][e];
           else if (a.bias != nullptr && n + e < a.n_out) v[0][e] += a.bias[n + e];
         }

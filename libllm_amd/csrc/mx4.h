@@ -30,10 +30,16 @@ typedef float f32x2_raw __attribute__((ext_vector_type(2)));
 // is 2^-127 and 255 NaN (checked on the device, tests/test_gpu_mx4.py).
 __device__ __forceinline__ float mx4_scale(uint32_t e) { return __uint_as_float(e << 23); }
 
-// The gate of the gated products, in 32 bits.  SiLU is finished before it meets the other factor: that
-// times the gate may overflow where the result does not (gate -1e20, up 1e20).
-__device__ __forceinline__ float mx4_gated(int act, float g, float u) {
-  return act == LLM_ACT_SILU ? u * (g / (1.0f + expf(-g))) : llm_gated(act, g, u);
+// The gate of the gated products, in 32 bits.  SiLU, g / (1 + e^-g), by h = e^(-|g| / 2): e^-g overflows for gates
+// below -88, whose products with a large up 32 bits still hold (gate -89, up 2^100: -2.5e-7), and up times the
+// gate may overflow where the result does not (gate -1e20, up 1e20); h does neither.  FINE: expf and a division, for
+// results in 32 bits; else the instructions for 2^x and 1 / x, within 2^-16 up to |g| = 100, for results that are
+// rounded to bfloat16 (2^-8).  Every kernel goes by that, so the sizes of a product change nothing.
+template <bool FINE> __device__ __forceinline__ float mx4_gated(int act, float g, float u) {
+  if (act != LLM_ACT_SILU) return llm_gated(act, g, u);
+  const float a = fabsf(g), h = FINE ? expf(-0.5f * a) : fast_exp2(-0.72134752f * a), d = 1.0f + h * h;
+  const float r = FINE ? 1.0f / d : __builtin_amdgcn_rcpf(d), t = g < 0.f ? h : 1.0f;
+  return (u * (t * r)) * (g * t);                          // (neither factor leaves the range before the result does)
 }
 
 // Eight codes, widened with their scale; exact (an element has two significant bits).
@@ -49,7 +55,7 @@ __device__ __forceinline__ Frag mx4_widen(uint32_t codes, float scale) {
   return u.f;
 }
 
-// C[16 x 16] += A[16 x 128] B[128 x 16] for two units; byte OA of `sa` and OB of `sb` are the scales.
+// C[16 x 16] += A[16 x 128] B[128 x 16], a unit of each; byte OA of `sa` and OB of `sb` are the scales.
 template <int OA, int OB>
 __device__ __forceinline__ f32x4 mx4_mfma(const uint4& a, uint32_t sa, const uint4& b, uint32_t sb, f32x4 c) {
   const i32x8_raw va = {(int)a.x, (int)a.y, (int)a.z, (int)a.w, 0, 0, 0, 0};

@@ -49,3 +49,30 @@ def test_the_same_of_weights_that_are_stored(ops, dtype, m, inter, act):
     x[:, 0], x[:, 1] = 1.0, 1.5
     got = ops.linear_swiglu(x.to(dtype).cuda(), w.to(dtype).cuda(), dtype, act).cpu()
     assert torch.isnan(got[:, [5, 7]]).all() and int(torch.isnan(got).sum()) == 2 * m
+
+
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("kernel", ["few", "many", "many, small", "joined"])
+def test_silu_of_gates_far_from_zero(ops, monkeypatch, kernel, out):
+    """Gates of -170 to 170 with ups of any size: the result is right wherever 32 bits hold it, though e^-g
+    overflows below -88 and its reciprocal is no normal number from -87 on."""
+    by_one_kernel(ops, monkeypatch, kernel)
+    inter, k = 48, 1024
+    w = torch.zeros((2 * inter, k))
+    w[:inter, 0] = 1.0
+    ups = [2.0 ** 100, 1.0, -2.0 ** -20]
+    for i in range(inter):
+        w[inter + i, 32 * (1 + i % 3)] = 1.0                    # (a block of its own each)
+    x = torch.zeros((341, k), dtype=torch.bfloat16)
+    x[:, 0] = torch.linspace(-170, 170, 341)
+    for i, up in enumerate(ups):
+        x[:, 32 * (1 + i)] = up
+    got = ops.linear_swiglu(x.cuda(), ops.quantize_mx4(w.cuda()), out).double().cpu().numpy()
+    g = x[:, :1].double().numpy()
+    want = g / (1 + np.exp(-g)) * np.array([ups[i % 3] for i in range(inter)])
+    # e^(-|g| / 2), twice: its argument, up to 0.73 |g|, is rounded twice where the instruction takes powers of
+    # two, |g| 2^-24 each time it is used; the rest are a dozen roundings of 2^-24 (an instruction's last bit is
+    # two of them).  Then the result's own; below 2^-126 it may be taken for zero.
+    half = 2.0 ** -8 if out == torch.bfloat16 else 2.0 ** -24
+    lim = (half + (2 * np.abs(g) + 16) * 2.0 ** -24) * np.abs(want) + 2.0 ** -126
+    assert (np.abs(got - want) <= lim).all(), np.abs(got - want).max()
