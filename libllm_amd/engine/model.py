@@ -76,15 +76,15 @@ class DecoderModel:
 
     def bind(self, tensors: Dict[str, torch.Tensor], ops, dtype) -> None:
         s = self.spec
-        per_part: Dict[int, Dict[str, torch.Tensor]] = {}
+        names: Dict[int, Dict[str, str]] = {}
         parts = {}
         for name, (part, rel, _decl) in self._collect().items():
             if part is None:
                 continue
-            per_part.setdefault(id(part), {})[rel] = tensors[name]
+            names.setdefault(id(part), {})[rel] = name
             parts[id(part)] = part
-        for pid, part in parts.items():
-            part.bind(per_part[pid], ops, dtype)
+        for pid, part in parts.items():                 # (tensors that are made when asked for live for one part's binding)
+            part.bind({rel: tensors[name] for rel, name in names[pid].items()}, ops, dtype)
         for block in self.blocks:                       # parts without tensors still get ops
             for part in [block.mixer, block.feed_forward] + list(block.norms):
                 if id(part) not in parts:

@@ -70,10 +70,10 @@ class Attention(Mixer):
     def weights(self):
         s = self.spec
         decl = {
-            s.q_name + ".weight": WeightDecl((self.q_dim, s.width)),
-            s.k_name + ".weight": WeightDecl((self.kv_dim, s.width)),
-            s.v_name + ".weight": WeightDecl((self.kv_dim, s.width)),
-            s.o_name + ".weight": WeightDecl((s.width, self.q_dim)),
+            s.q_name + ".weight": WeightDecl((self.q_dim, s.width), low_bit=True),
+            s.k_name + ".weight": WeightDecl((self.kv_dim, s.width), low_bit=True),
+            s.v_name + ".weight": WeightDecl((self.kv_dim, s.width), low_bit=True),
+            s.o_name + ".weight": WeightDecl((s.width, self.q_dim), low_bit=True),
         }
         if s.qkv_bias:
             decl[s.q_name + ".bias"] = WeightDecl((self.q_dim,), role="vector", init="normal")

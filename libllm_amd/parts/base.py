@@ -26,10 +26,13 @@ class WeightDecl:
     or the whole model runs in 32-bit).  role "vector": small per-channel values (norm scales,
     biases) held in float32 on the device.  role "table": integer table held as int32.
     ``init`` says how the random-weights mode fills it: "normal", "ones" or "zeros".
+    ``low_bit``: a matrix that its part holds in fewer bits where a model's weights are asked for
+    in such a format; it is then handed over as the file stores it, to be rounded once.
     """
     shape: Tuple[int, ...]
     role: str = "matrix"
     init: str = "normal"
+    low_bit: bool = False
 
 
 @dataclass(frozen=True)

@@ -45,9 +45,9 @@ class SwiGLU(FeedForward):
     def weights(self):
         s = self.spec
         return {
-            s.gate_name + ".weight": WeightDecl((s.intermediate, s.width)),
-            s.up_name + ".weight": WeightDecl((s.intermediate, s.width)),
-            s.down_name + ".weight": WeightDecl((s.width, s.intermediate)),
+            s.gate_name + ".weight": WeightDecl((s.intermediate, s.width), low_bit=True),
+            s.up_name + ".weight": WeightDecl((s.intermediate, s.width), low_bit=True),
+            s.down_name + ".weight": WeightDecl((s.width, s.intermediate), low_bit=True),
         }
 
     def bind(self, tensors, ops, dtype):

@@ -8,7 +8,7 @@ from .engine.model import DecoderModel
 from .engine.step import Engine
 from .errors import ConfigError
 from .weights import load_tensors, random_tensors
-from .weights.loader import place
+from .weights.loader import Tensors, place
 
 _DTYPES = {"bfloat16": torch.bfloat16, "bf16": torch.bfloat16,
            "float32": torch.float32, "fp32": torch.float32}
@@ -33,8 +33,7 @@ def default_ops():
 WEIGHT_FORMATS = ("stored", "mxfp4")
 
 
-def _bind(model, tensors, ops, dtype, weights):
-    """Binds the tensors, the layers' matrices in the format asked for."""
+def _check_format(weights, ops, dtype):
     if weights not in WEIGHT_FORMATS:
         raise ConfigError("weights are %s, not %r" % (" or ".join(WEIGHT_FORMATS), weights))
     if weights == "mxfp4":
@@ -42,6 +41,10 @@ def _bind(model, tensors, ops, dtype, weights):
             raise ConfigError("weights in MXFP4 need bfloat16 activations")
         if not hasattr(ops, "quantize_mx4"):
             raise ConfigError("these operations know no weights in MXFP4")
+
+
+def _bind(model, tensors, ops, dtype, weights):
+    """Binds the tensors, the layers' matrices in the format asked for."""
     before = getattr(ops, "weight_format", None)
     ops.weight_format = weights
     try:
@@ -58,17 +61,18 @@ def load_engine(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, ops=No
     bfloat16 mode a matrix that the file stores in 32-bit stays float32 (true 32-bit products
     for it) instead of becoming bfloat16.  ``tiled_weights=False``: no second, tiled copy of the
     bfloat16 matrices (half the weight memory; decoding is 5 to 11 % slower).  ``weights="mxfp4"``:
-    the matrices of attention and feed-forwards are rounded to MXFP4 when they are bound (4.25 bits
-    an element, held once; the embedding and the output matrix stay as they are)."""
+    the matrices of attention and feed-forwards are rounded to MXFP4 when they are bound, from what the
+    file stores (4.25 bits an element, held once; the embedding and the output matrix are as without)."""
     config = config_from_dir(model_dir)
     tdtype = parse_dtype(dtype)
     spec = config.to_spec()
     model = DecoderModel(spec)
     ops = ops if ops is not None else default_ops()
+    _check_format(weights, ops, tdtype)
     if not tiled_weights:
         ops.pack_weights = False
     tensors = load_tensors(model_dir, model.declared(), spec.optional_tensors, tdtype, ops.device,
-                           keep_float32)
+                           keep_float32, weights)
     _bind(model, tensors, ops, tdtype, weights)
     engine = Engine(model, ops, tdtype, max_tokens, max_slots=max_slots, use_graphs=use_graphs)
     engine.config = config
@@ -87,14 +91,16 @@ def random_engine(config, seed: int = 0, dtype="bfloat16", max_tokens: int = 819
     spec = config.to_spec()
     model = DecoderModel(spec)
     ops = ops if ops is not None else default_ops()
+    _check_format(weights, ops, tdtype)
     if not tiled_weights:
         ops.pack_weights = False
     declared = model.declared()
-    tensors = {}
+    tensors = Tensors()
     for name in sorted(declared):
-        t = random_tensors({name: declared[name]}, seed, std=std, dtype=stored,
-                           device=ops.device)[name]
-        tensors[name] = place(t, declared[name], tdtype, ops.device)
+        def draw(name=name, decl=declared[name]):
+            t = random_tensors({name: decl}, seed, std=std, dtype=stored, device=ops.device)[name]
+            return place(t, decl, tdtype, ops.device, weights=weights)
+        tensors[name] = draw if weights != "stored" and declared[name].low_bit else draw()
     _bind(model, tensors, ops, tdtype, weights)
     engine = Engine(model, ops, tdtype, max_tokens, max_slots=max_slots, use_graphs=use_graphs)
     engine.config = config

@@ -11,7 +11,8 @@ file costs no more memory than a 16-bit one; small per-channel vectors (norm sca
 held in float32, which is how a vector stored in 32-bit stays so; integer tables become int32.
 With ``keep_float32`` a matrix stored in 32-bit or wider stays float32 in bfloat16 mode too, and
 its products then run in true 32-bit.  With dtype float32 every floating tensor is widened to
-32-bit and nothing is rounded on the way.
+32-bit and nothing is rounded on the way.  A matrix that its part will round to fewer bits comes as
+the file stores it, in bfloat16 or else float32 (64 bits are rounded to that): it is rounded once.
 """
 import fnmatch
 from typing import Dict, Iterable
@@ -68,33 +69,48 @@ def check_tensors(entries: Dict[str, TensorEntry], expected: Dict[str, WeightDec
     raise err
 
 
+class Tensors(dict):
+    """Tensors by name; a value may be a function that makes the tensor when it is asked for, so
+    that a wide copy of a matrix lives no longer than its part takes to round it."""
+
+    def __getitem__(self, name):
+        t = super().__getitem__(name)
+        return t() if callable(t) else t
+
+
 def device_dtype(decl: WeightDecl, stored: torch.dtype, model_dtype: torch.dtype,
-                 keep_float32: bool = False) -> torch.dtype:
+                 keep_float32: bool = False, weights: str = "stored") -> torch.dtype:
     if decl.role == "table":
         return torch.int32
     if decl.role == "vector" or model_dtype == torch.float32:
         return torch.float32
+    if weights != "stored" and decl.low_bit:
+        return torch.bfloat16 if stored == torch.bfloat16 else torch.float32
     if keep_float32 and stored in (torch.float32, torch.float64):
         return torch.float32
     return torch.bfloat16
 
 
 def place(t: torch.Tensor, decl: WeightDecl, model_dtype: torch.dtype, device,
-          keep_float32: bool = False) -> torch.Tensor:
-    target = device_dtype(decl, t.dtype, model_dtype, keep_float32)
+          keep_float32: bool = False, weights: str = "stored") -> torch.Tensor:
+    target = device_dtype(decl, t.dtype, model_dtype, keep_float32, weights)
     if decl.role == "table" and t.numel() and (int(t.max()) > 2**31 - 1 or int(t.min()) < -2**31):
         raise WeightError("an integer table holds values outside the int32 range")
     return t.to(device=device, dtype=target, copy=True).contiguous()
 
 
 def load_tensors(model_dir: str, expected: Dict[str, WeightDecl], optional: Iterable[str],
-                 model_dtype: torch.dtype, device, keep_float32: bool = False) -> Dict[str, torch.Tensor]:
+                 model_dtype: torch.dtype, device, keep_float32: bool = False,
+                 weights: str = "stored") -> Dict[str, torch.Tensor]:
+    """``weights``: the format the model's parts hold their matrices in; those that are rounded to
+    it are read when they are asked for."""
     entries = open_model_files(model_dir)
     check_tensors(entries, expected, optional)
-    out = {}
+    out = Tensors()
     for name, decl in expected.items():
-        e = entries[name]
-        out[name] = place(e.file.tensor(name), decl, model_dtype, device, keep_float32)
+        def read(name=name, decl=decl, file=entries[name].file):
+            return place(file.tensor(name), decl, model_dtype, device, keep_float32, weights)
+        out[name] = read if weights != "stored" and decl.low_bit else read()
     for f in {e.file for e in entries.values()}:
         f.close()
     return out

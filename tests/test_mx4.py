@@ -100,3 +100,47 @@ def test_a_matrix_is_bound_once_whatever_its_order():
     part = Linear(12, 24, low_bit=True)
     part.bind(w.t()[:24], ops=Ops(), like=whole.prepared)
     assert torch.equal(part.prepared.w, w.t()[:24])
+
+
+@pytest.mark.parametrize("stored", ["float32", "float16", "bfloat16", "float64"])
+def test_matrices_come_to_the_quantiser_as_the_file_stores_them(tmp_path, stored):
+    """Rounded to bfloat16 first they would be rounded twice; what is held in the model's type is so as ever."""
+    import os
+
+    from libllm_amd.config import config_from_dict
+    from libllm_amd.engine import DecoderModel
+    from libllm_amd.runtime import _bind, load_tensors
+    from plain import files
+    from tiny import TINY_A, make_model
+
+    class Held:
+        def leading_rows(self, rows):
+            return self
+
+    class Ops:
+        device = torch.device("cpu")
+
+        def __init__(self):
+            self.given = []
+
+        def quantize_mx4(self, w):
+            self.given.append(w)
+            return Held()
+    path = make_model(tmp_path, TINY_A, seed=3, stored=stored)
+    held = files.read_safetensors(os.path.join(path, "model.safetensors"))
+    model, ops = DecoderModel(config_from_dict(TINY_A).to_spec()), Ops()
+    tensors = load_tensors(path, model.declared(), model.spec.optional_tensors, torch.bfloat16, ops.device,
+                           weights="mxfp4")
+    _bind(model, tensors, ops, torch.bfloat16, "mxfp4")
+    for i in range(len(model.blocks)):
+        at = "model.layers.%d." % i
+        for names in (("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj"), ("self_attn.o_proj",),
+                      ("mlp.gate_proj", "mlp.up_proj"), ("mlp.down_proj",)):
+            w = torch.cat([torch.from_numpy(held[at + n + ".weight"]).double() for n in names])
+            if stored == "float64":
+                w = w.float().double()
+            match = [g for g in ops.given if g.shape == w.shape and torch.equal(g.double(), w)]
+            assert len(match) == 1 and match[0].dtype == (torch.bfloat16 if stored == "bfloat16" else torch.float32)
+    assert len(ops.given) == 4 * len(model.blocks)
+    assert tensors["model.embed_tokens.weight"].dtype == torch.bfloat16
+    assert tensors["model.norm.weight"].dtype == torch.float32
