@@ -43,14 +43,20 @@ def _check_format(weights, ops, dtype):
             raise ConfigError("these operations know no weights in MXFP4")
 
 
+class _Binding:
+    """The operations as a model's parts see them while they are bound: with the format of this
+    model's weights, which another model that is bound over them at the same time does not share."""
+
+    def __init__(self, ops, weights):
+        self._ops, self.weight_format = ops, weights
+
+    def __getattr__(self, name):
+        return getattr(self._ops, name)
+
+
 def _bind(model, tensors, ops, dtype, weights):
     """Binds the tensors, the layers' matrices in the format asked for."""
-    before = getattr(ops, "weight_format", None)
-    ops.weight_format = weights
-    try:
-        model.bind(tensors, ops, dtype)
-    finally:
-        ops.weight_format = before
+    model.bind(tensors, _Binding(ops, weights), dtype)
 
 
 def load_engine(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, ops=None,

@@ -144,3 +144,56 @@ def test_matrices_come_to_the_quantiser_as_the_file_stores_them(tmp_path, stored
     assert len(ops.given) == 4 * len(model.blocks)
     assert tensors["model.embed_tokens.weight"].dtype == torch.bfloat16
     assert tensors["model.norm.weight"].dtype == torch.float32
+
+
+def test_two_models_bound_at_once_over_the_same_operations(tmp_path):
+    """Each in its own format, whatever the other asks for between the two's matrices."""
+    import threading
+
+    from libllm_amd.config import config_from_dict
+    from libllm_amd.engine import DecoderModel
+    from libllm_amd.runtime import _bind, load_tensors
+    from tiny import TINY_A, make_model
+
+    class Held:
+        def leading_rows(self, rows):
+            return self
+
+    class Ops:
+        device = torch.device("cpu")
+        turns = threading.Barrier(2, timeout=60)
+
+        def wait(self):                     # the two threads take every matrix of a layer in step
+            try:
+                self.turns.wait()
+            except threading.BrokenBarrierError:
+                pass
+
+        def quantize_mx4(self, w):
+            self.wait()
+            return Held()
+
+        def prepare_weight(self, w, like=None):
+            if like is None and w.shape[0] != 256:
+                self.wait()
+            return w
+    path, ops, models = make_model(tmp_path, TINY_A, seed=3), Ops(), {}
+
+    def load(weights):
+        try:
+            model = DecoderModel(config_from_dict(TINY_A).to_spec())
+            _bind(model, load_tensors(path, model.declared(), model.spec.optional_tensors, torch.bfloat16, ops.device,
+                                      weights=weights), ops, torch.bfloat16, weights)
+            models[weights] = model
+        finally:
+            ops.turns.abort()
+    threads = [threading.Thread(target=load, args=(w,)) for w in ("mxfp4", "stored")]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for weights in ("mxfp4", "stored"):
+        for block in models[weights].blocks:
+            for linear in (block.mixer.qkv, block.mixer.out, block.feed_forward.gate_up, block.feed_forward.down):
+                assert isinstance(linear.prepared, Held) == (weights == "mxfp4")
+    assert not hasattr(ops, "weight_format")
