@@ -446,6 +446,9 @@ def main() -> int:
     if args.gpus != 1:
         print("bench.py measures one GPU only: this library does not run on several (--gpus %d)" % args.gpus)
         return 2
+    if args.weights != "stored" and (args.workload or args.sweep or args.unequal or args.requests):
+        ap.error("--weights %s is for the decode steps of the default run, not for --workload, --sweep, --unequal or --requests"
+                 % args.weights)
 
     import torch
 

@@ -197,3 +197,14 @@ def test_two_models_bound_at_once_over_the_same_operations(tmp_path):
             for linear in (block.mixer.qkv, block.mixer.out, block.feed_forward.gate_up, block.feed_forward.down):
                 assert isinstance(linear.prepared, Held) == (weights == "mxfp4")
     assert not hasattr(ops, "weight_format")
+
+
+@pytest.mark.parametrize("mode", [["--workload", "batch64"], ["--sweep"], ["--unequal"], ["--requests", "8"]])
+def test_bench_measures_mxfp4_in_the_default_run_only(mode):
+    """The other runs build engines with stored weights: they do not pass for what was asked."""
+    import os
+    import subprocess
+    import sys
+    bench = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "bench.py")
+    got = subprocess.run([sys.executable, bench, "--weights", "mxfp4"] + mode, capture_output=True, text=True, timeout=100)
+    assert got.returncode == 2 and "--weights mxfp4" in got.stderr and not got.stdout
