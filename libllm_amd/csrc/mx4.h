@@ -42,7 +42,8 @@ template <bool FINE> __device__ __forceinline__ float mx4_gated(int act, float g
   return (u * (t * r)) * (g * t);                          // (neither factor leaves the range before the result does)
 }
 
-// Eight codes, widened with their scale; exact (an element has two significant bits).
+// Eight codes, widened with their scale; exact (an element has two significant bits), subnormal numbers too, but
+// for numbers of 2^128 and more, which only scale bytes of 253 and 254 reach: they become infinities.
 __device__ __forceinline__ Frag mx4_widen(uint32_t codes, float scale) {
   union {
     Frag f;

@@ -122,7 +122,8 @@ class Mx4Ops:
         return q
 
     def dequantize_mx4(self, q: Mx4Matrix, dtype=torch.bfloat16) -> torch.Tensor:
-        """The numbers that ``q`` stands for, exactly (a scale above 2^125 can give an infinity)."""
+        """The numbers that ``q`` stands for, exactly (with a scale of 2^126 or 2^127 those of 2^128 and more
+        are infinities)."""
         self._mx4(q, "the matrix to read")
         code = self._dtype_code(dtype)
         m, k = q.shape
@@ -134,7 +135,8 @@ class Mx4Ops:
         """A matrix that is in MXFP4 already, as files hold it: ``codes`` uint8
         ``[rows, ceil(width / 2)]`` or wider, two elements a byte, the even one in the low half, and
         ``scales`` uint8 ``[rows, ceil(width / 32)]``.  ``width``: twice the columns of ``codes``
-        unless it is given (an odd width, padded rows)."""
+        unless it is given (an odd width, padded rows).  Every byte is taken; of scales of 253 and 254
+        ``linear`` says what becomes."""
         if codes.dtype != torch.uint8 or scales.dtype != torch.uint8:
             raise KernelError("mx4_from_codes: codes and scales are matrices of uint8")
         self._matrix(codes, "the matrix of codes")

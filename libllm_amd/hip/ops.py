@@ -536,7 +536,9 @@ class HipOps(Mx4Ops):
 
     def linear(self, x, w, bias, out_dtype, residual=None, then_norm=None):
         """x W^T (+ bias) as ``out_dtype``.  ``x`` is a matrix or a ``normed`` record; with a weight
-        in MXFP4 (``quantize_mx4``, ``mx4_from_codes``) it may be in MXFP4 too.  With
+        in MXFP4 (``quantize_mx4``, ``mx4_from_codes``) it may be in MXFP4 too.  (A number of 2^128 or
+        more, which scale bytes of 253 and 254 alone can stand for, is an infinity to a matrix in
+        bfloat16, as ``dequantize_mx4`` reads it; with both in MXFP4 it is what it is.)  With
         ``residual`` (the float32 stream, same shape as the result) the product is added into it
         where the kernel can do that, and None is returned; otherwise the result is returned and
         the caller adds it.  ``then_norm`` = (weight, eps) says that an RMS norm with these reads
