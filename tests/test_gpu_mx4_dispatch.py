@@ -162,6 +162,86 @@ def test_bands_of_blocks(ops, monkeypatch, m, n, k, ks, four, form):
     assert ((got.double() - relu.double()).abs() <= 2.0 ** -7 * relu.double().abs()).all()
 
 
+# outputs of the product for few rows: tiles for half of 256 units at most, up to one a unit, up to three, and
+# more, odd numbers of them, and a last one that is not whole
+FEW_OUTPUTS = [1000, 2504, 4200, 12392]
+FEW_ROWS = [1, 4, 6, 12, 16, 20, 32, 40]
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("k", [64, 300, 2100])
+@pytest.mark.parametrize("n", FEW_OUTPUTS)
+def test_few_rows(ops, launched, monkeypatch, n, k, four):
+    monkeypatch.setattr(ops, "_mx4_plan", lambda *sizes: (-1, 1))
+    w, wd = held(ops, n, k, n)
+    bias = whole((n,), 3).float()
+    for m in FEW_ROWS:
+        x = whole((m, k), m)
+        rows, want = rows_for(ops, x, four), x.double() @ wd.t()
+        for out in (torch.float32, torch.bfloat16):
+            assert torch.equal(ops.linear(rows, w, None, out), want.to(out)), (m, out)
+        assert torch.equal(ops.linear(rows, w, bias, torch.float32).double(), want + bias.double()), m
+    assert FEW in dict(launched) and not forms(launched)
+
+
+@pytest.mark.parametrize("act", ["silu", "relu"])
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("k", [64, 300, 2100])
+@pytest.mark.parametrize("inter", [1008, 2512, 4208, 12400])
+def test_few_rows_gated(ops, launched, monkeypatch, inter, k, four, act):
+    monkeypatch.setattr(ops, "_mx4_plan", lambda *sizes: (-1, 1))
+    w, wd = held(ops, 2 * inter, k, inter)
+    for m in FEW_ROWS:
+        x = whole((m, k), m) * 2.0 ** -5
+        y = x.double() @ wd.t()
+        g, u = y[:, :inter], y[:, inter:]
+        want = g.clamp(min=0) * u if act == "relu" else g * torch.sigmoid(g) * u
+        got = ops.linear_swiglu(rows_for(ops, x, four), w, None, act).double()
+        lim = 2.0 ** -16 * (g * u).abs()                         # as for many rows
+        assert ((got - want).abs() <= lim + 2.0 ** -8 * (want.abs() + lim)).all(), m
+    assert FEW in dict(launched) and not forms(launched) and JOIN not in dict(launched)
+
+
+@pytest.mark.parametrize("n,k", [(2504, 1056), (4200, 1056), (12392, 520)])
+def test_a_row_is_the_same_whatever_the_batch(ops, n, k):
+    """The same bits, whichever variant of the product for few rows the sizes choose."""
+    x = normal((32, k), 8, dtype=torch.bfloat16).cuda()
+    q = ops.quantize_mx4(normal((n, k), 9, dtype=torch.bfloat16).cuda())
+    both = ops.quantize_mx4(normal((2 * 2512, k), 9, dtype=torch.bfloat16).cuda())
+    product, gated = ops.linear(x, q, None, torch.float32), ops.linear_swiglu(x, both)
+    for m0, m in ((0, 1), (3, 4), (5, 7), (16, 16), (10, 9), (10, 22), (1, 31)):
+        assert torch.equal(ops.linear(x[m0:m0 + m], q, None, torch.float32), product[m0:m0 + m])
+        assert torch.equal(ops.linear_swiglu(x[m0:m0 + m], both), gated[m0:m0 + m])
+    for m in (1, 16, 17, 31):                                    # (rows in MXFP4 begin at whole tiles)
+        assert torch.equal(ops.linear(ops.quantize_mx4(x[:m]), q, None, torch.float32),
+                           ops.linear(ops.quantize_mx4(x), q, None, torch.float32)[:m])
+
+
+@pytest.mark.parametrize("m", [1, 6, 12, 16, 30])
+@pytest.mark.parametrize("n,k", [(2512, 96), (4208, 200), (12400, 300)])
+def test_few_rows_added_into_the_stream(ops, launched, m, n, k):
+    x, (w, wd), res = whole((m, k), m), held(ops, n, k, n), whole((m, n), 5).float()
+    want = res.double() + x.double() @ wd.t()
+    del launched[:]
+    assert ops.linear(x, w, None, torch.bfloat16, residual=res) is None
+    assert FEW in dict(launched) and not forms(launched) and torch.equal(res.double(), want)
+
+
+@pytest.mark.parametrize("m", [1, 6, 12, 16])
+@pytest.mark.parametrize("n,k,inter", [(2512, 96, 528), (4208, 96, 528), (12400, 200, 528), (96, 64, 2512),
+                                       (96, 64, 4208), (96, 64, 12400)])
+def test_norm_between_two_wide_products(ops, m, n, k, inter):
+    mx4.test_norm_between_two_products(ops, m, n, k, inter)
+
+
+@pytest.mark.parametrize("bias,write,rot_half", [(True, True, True), (False, False, False)])
+@pytest.mark.parametrize("n_heads,n_kv,hd", [(153, 2, 16), (259, 2, 16), (96, 2, 48), (771, 2, 16)])
+@pytest.mark.parametrize("seqs", [[(0, 0, 1)], [(i, 7 * i, 1) for i in range(12)], [(1, 60, 9), (0, 5, 15)]])
+def test_wide_stacked_projection_of_few_rows(ops, launched, n_heads, n_kv, hd, seqs, bias, write, rot_half):
+    mx4.test_stacked_projection(ops, n_heads, n_kv, hd, 96, seqs, bias, write, rot_half)
+    assert "llm_gemm_mx4_rows_rope" in dict(launched) and not forms(launched)
+
+
 def run_of(ops, weights, nw, h, res):
     """A run of a layer's products: into the stream in slices of K, its norm, gate and up, and down."""
     down, gate_up = weights
