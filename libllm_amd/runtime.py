@@ -56,7 +56,7 @@ class _Binding:
 
 def _bind(model, tensors, ops, dtype, weights):
     """Binds the tensors, the layers' matrices in the format asked for."""
-    model.bind(tensors, _Binding(ops, weights), dtype)
+    model.bind(tensors, ops if weights == "stored" else _Binding(ops, weights), dtype)
 
 
 def load_engine(model_dir: str, dtype="bfloat16", max_tokens: int = 8192, ops=None,
