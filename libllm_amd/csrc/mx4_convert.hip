@@ -201,7 +201,8 @@ __global__ __launch_bounds__(256) void mx4_dequantize_kernel(const uint32_t* __r
 }
 
 // Codes [N, ldc] bytes (two elements a byte, the even one low) and scales [N, ceil(K / 32)] as a
-// file holds them, into the tiles.
+// file holds them, into the tiles.  Once for a weight: sixteen loads of a byte a lane, whatever rows are aligned to
+// (28,672 x 4,096: 107 us, 1.2 TB/s).
 __global__ __launch_bounds__(256) void mx4_pack_kernel(const uint8_t* __restrict__ rows, size_t ldc,
                                                        const uint8_t* __restrict__ row_scales, int N, int K,
                                                        uint4* __restrict__ codes, uint32_t* __restrict__ scales,

@@ -37,8 +37,9 @@ def tiled_sizes(rows: int, width: int):
 
 class Mx4Matrix:
     """A matrix ``[rows, width]`` in MXFP4: ``codes`` and ``scales`` are flat uint8 tensors in the
-    order the matrix cores read them, zero where rows and columns are filled up.  What ``HipOps.quantize_mx4`` and ``HipOps.mx4_from_codes``
-    return, and the products take as a weight, or on both sides."""
+    order the matrix cores read them, zero where rows and columns are filled up.  What
+    ``HipOps.quantize_mx4`` and ``HipOps.mx4_from_codes`` return, and the products take as a weight, or
+    on both sides."""
     dtype = "mxfp4"
     __slots__ = ("shape", "device", "codes_ptr", "scales_ptr", "_storage")
 
@@ -113,7 +114,7 @@ class Mx4Ops:
         """The matrix ``x`` (bfloat16 or float32, rows contiguous; they may lie further apart than
         their length) in MXFP4.  The scale of a block is 2^(floor(log2(max |x|)) - 2), at least
         2^-127; an element is divided by it and rounded to the nearest code, ties to the even one,
-        6 beyond 6.  A block that holds an infinity or a NaN reads as NaN."""
+        6 beyond 6.  A block that holds an infinity or a NaN reads as NaN.  A matrix without rows is refused."""
         self._matrix(x, "the matrix to quantise")
         m, k = x.shape
         q = self._mx4_empty(m, k)
@@ -161,7 +162,9 @@ class Mx4Ops:
 
     # ---- products
     def _mx4_few(self, m, n, k, four):
-        """Whether the product goes to the kernel for few rows.  Up to 32 rows always (us, 32 rows, that
+        """Whether the product goes to the kernel for few rows (times of plain products over warm weights; over
+        cold ones, with the stream or the cache to write, 64 rows of K 4,096 take 14.5 us for 4,096 outputs and 16.3
+        for 6,144).  Up to 32 rows always (us, 32 rows, that
         kernel against the other: K 14,336, 4,096 outputs 19.5 against 23.0, gate and up of 4,096 x 14,336
         22.7 against 22.8).  Up to 64, where it reads W twice, if W is small and has two tiles a compute
         unit at most (MXFP4: one and a half), so that the other cannot fill the units (64 rows, bfloat16:
@@ -183,7 +186,7 @@ class Mx4Ops:
     # The product for many rows, by form (csrc/gemm_mx4_many.hip): rows of X and of W a block, the us that
     # 128 elements of K take with one, two, three, four blocks a compute unit (beyond, as much again for
     # every four), and as how many such elements more a block's begin and end count.  Fitted to 135
-    # products of each kind, 128 to 14,336 elements of K, 64 to 4,096 rows, 2,048 to 28,672 outputs, in every
+    # products of each kind (warm weights, plain epilogue), 128 to 14,336 elements of K, 64 to 4,096 rows, 2,048 to 28,672 outputs, in every
     # form: what this says is best takes 0.1 % longer than the best on average, 4 % at most.
     _MX4_FORMS = {
         False: ((0, 256, 256, (2.56, 5.12, 7.68, 10.24), 1.5), (1, 128, 256, (1.255, 2.51, 3.765, 5.02), 4.5),
