@@ -310,3 +310,36 @@ def test_many_rows_from_two_threads(ops, launched):
     for name in "ab":
         for a, b in zip(want, got[name]):
             assert all(torch.equal(p, q) for p, q in zip(a, b))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,width", [(131090, 16400), (131089, 16403)])
+def test_conversions_of_more_elements_than_32_bits_count(ops, rows, width, dtype):
+    """Offsets of elements, of codes and of what is read back pass 2^31; the last rows are what they are alone."""
+    assert rows * width > 1 << 31
+    x = torch.empty((rows, width), dtype=dtype, device="cuda")
+    x.copy_(whole((rows, 1), 1).to(dtype) * torch.arange(1, width + 1, device="cuda").remainder(7).to(dtype) * 0.25)
+    q = ops.quantize_mx4(x)
+    back = ops.dequantize_mx4(q, dtype)
+    at = rows // 16 * 16
+    for first, last in ((0, 48), (at - 48, rows)):
+        part = ops.quantize_mx4(x[first:last].contiguous())
+        assert torch.equal(ops.dequantize_mx4(part, dtype), back[first:last])
+    codes, scales = ops.quantize_mx4(x[at - 16:at].contiguous()), q.leading_rows(at)
+    assert torch.equal(scales.codes[-codes.codes.numel():], codes.codes)
+    assert torch.equal(scales.scales[-codes.scales.numel():], codes.scales)
+
+
+@pytest.mark.parametrize("four", [False, True])
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("m,n", [(33000, 65600), (33001, 65603)])
+def test_results_of_more_elements_than_32_bits_count(ops, launched, m, n, out, four):
+    assert m * n > 1 << 31
+    k = 64
+    x, (w, wd) = whole((m, k), 1), held(ops, n, k, 2)
+    rows = rows_for(ops, x, four)
+    got = ops.linear(rows, w, None, out)
+    assert forms(launched)
+    for first in list(range(0, m - 500, 4096)) + [m - 500]:
+        want = (x[first:first + 500].double() @ wd.t()).to(out)
+        assert torch.equal(got[first:first + 500], want), first
